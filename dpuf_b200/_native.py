@@ -41,6 +41,10 @@ CUDA_SOURCES = [
     "ops_had_asym.cu",
     "noalloc.cu",
     "sampling.cu",
+    "kernels_rope.cu",
+    "kernels_paged_attn.cu",
+    "kernels_sample.cu",
+    "ops_serving.cu",
 ]
 
 

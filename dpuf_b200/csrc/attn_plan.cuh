@@ -1,0 +1,176 @@
+// attn_plan.cuh - how the paged attention kernels share their work out.
+//
+// An item is a tile of rows of one sequence and KV head: row r of a sequence is query head
+// kv_head * group + r % group of its new token r / group, so all query heads that read a KV head
+// sit in the same tiles and its keys are read once for them.  An item walks the key blocks that
+// its rows see.  All items' key blocks, laid end to end, are cut into equal runs, one per CTA,
+// so that a few long sequences fill the GPU as well as many short ones and ragged batches stay
+// balanced; the lengths are read on the device, and the host never waits for them.  An item that
+// crosses a cut is computed in parts: each CTA leaves its part's running maximum, sum and
+// unnormalised output in the workspace, and the CTA that arrives last (a counter per item, no
+// waiting) joins the parts in the order of their keys, so results do not depend on timing.
+//   part of an item that began in an earlier CTA: slot 2c; part that a later CTA goes on with:
+//   slot 2c + 1; the counter is that of the CTA in which the item begins.
+#pragma once
+#include "serving.cuh"
+
+namespace dpuf {
+
+constexpr int kAttnMaxCtas = 148 * 4;
+constexpr int kAttnCounterBytes = (kAttnMaxCtas * 4 + 255) & ~255;
+
+struct AttnArgs {
+  DpufPagedAttentionArgs a;
+  int group;    // query heads per KV head
+  int max_kv;   // positions that a page table row can hold
+  int page_shift;
+};
+
+struct AttnSeq {
+  int q0, qn, kv;  // first new token, new tokens, stored positions
+};
+
+DPUF_DEV AttnSeq attn_seq(const AttnArgs& p, int s) {
+  AttnSeq i;
+  i.q0 = min(max(p.a.q_start[s], 0), p.a.n_tokens);
+  i.qn = min(min(max(p.a.q_start[s + 1] - i.q0, 0), p.a.n_tokens - i.q0), p.a.max_q);
+  i.kv = min(max(p.a.kv_len[s], 0), p.max_kv);
+  return i;
+}
+
+// Positions that the tokens [t0, t1] of a sequence see between them.
+DPUF_DEV void attn_span(const AttnArgs& p, const AttnSeq& q, int t0, int t1, int* lo, int* hi) {
+  const int first = q.kv - q.qn + t0, last = q.kv - q.qn + t1;
+  *hi = p.a.causal ? min(max(last + 1, 0), q.kv) : q.kv;
+  *lo = p.a.window > 0 ? max(first - p.a.window + 1, 0) : 0;
+}
+
+// Key blocks [*blk0, *blk0 + n) of tile `tile` (at least one, so that rows that see nothing are
+// written too).
+template <int BM, int BN>
+DPUF_DEV int attn_tile_blocks(const AttnArgs& p, const AttnSeq& q, int tile, int* blk0) {
+  int lo, hi;
+  attn_span(p, q, tile * BM / p.group, min(q.qn - 1, (tile * BM + BM - 1) / p.group), &lo, &hi);
+  *blk0 = lo / BN;
+  return max((hi + BN - 1) / BN - *blk0, 1);
+}
+
+template <int BM>
+DPUF_DEV int attn_tiles(const AttnArgs& p, const AttnSeq& q) {
+  return (q.qn * p.group + BM - 1) / BM;
+}
+
+// A place in the sequence of all key blocks.
+struct AttnCursor {
+  AttnSeq seq;
+  int s, head, tile, tiles;
+  int blk0, n_blk;    // the item's key blocks
+  int at;             // block within the item
+  long long begin;    // the item's first block in the sequence of all
+};
+
+template <int BM, int BN>
+DPUF_DEV void attn_next_item(const AttnArgs& p, AttnCursor& c) {
+  c.begin += c.n_blk;
+  c.at = 0;
+  if (++c.tile == c.tiles) {
+    c.tile = 0;
+    if (++c.head == p.a.kv.n_kv) {
+      c.head = 0;
+      do {
+        if (++c.s >= p.a.n_seqs) return;
+        c.seq = attn_seq(p, c.s);
+        c.tiles = attn_tiles<BM>(p, c.seq);
+      } while (c.tiles == 0);
+    }
+  }
+  c.n_blk = attn_tile_blocks<BM, BN>(p, c.seq, c.tile, &c.blk0);
+}
+
+struct AttnShare {  // in shared memory
+  AttnCursor start;
+  long long total;
+  long long warp_sum[32];
+};
+
+struct AttnRun {  // this CTA's run of key blocks
+  AttnCursor cur;
+  long long total;  // blocks of all items
+  int n;            // blocks of this CTA (0: nothing to do)
+  int ctas;         // CTAs that have blocks
+};
+
+// All threads of the CTA call this together.
+template <int BM, int BN>
+DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x;
+  const int per = (p.a.n_seqs + nt - 1) / nt;
+  const int s0 = min(tid * per, p.a.n_seqs), s1 = min(s0 + per, p.a.n_seqs);
+  auto cost = [&](const AttnSeq& q) {
+    long long c = 0;
+    int b0;
+    for (int t = 0, n = attn_tiles<BM>(p, q); t < n; t++) c += attn_tile_blocks<BM, BN>(p, q, t, &b0);
+    return c;
+  };
+  long long mine = 0;
+  for (int s = s0; s < s1; s++) mine += cost(attn_seq(p, s)) * p.a.kv.n_kv;
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(kFull, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh.warp_sum[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < (nt >> 5); w++) {
+    if (w < warp) before += sh.warp_sum[w];
+    total += sh.warp_sum[w];
+  }
+  incl += before;
+  AttnRun r;
+  r.total = total;
+  r.ctas = (int)min((long long)ctas, total);
+  r.n = 0;
+  if (cta >= r.ctas) return r;  // the whole CTA
+  const long long b = total * cta / r.ctas, e = total * (cta + 1) / r.ctas;
+  r.n = (int)(e - b);
+  if (b >= incl - mine && b < incl) {  // one thread
+    long long at = incl - mine;
+    AttnCursor c;
+    for (int s = s0; s < s1; s++) {
+      c.seq = attn_seq(p, s);
+      const long long k = cost(c.seq);
+      if (b < at + k * p.a.kv.n_kv) {
+        c.s = s;
+        c.head = (int)((b - at) / k);
+        at += c.head * k;
+        c.tiles = attn_tiles<BM>(p, c.seq);
+        for (c.tile = 0;; c.tile++) {
+          c.n_blk = attn_tile_blocks<BM, BN>(p, c.seq, c.tile, &c.blk0);
+          if (b < at + c.n_blk) break;
+          at += c.n_blk;
+        }
+        c.begin = at;
+        c.at = (int)(b - at);
+        break;
+      }
+      at += k * p.a.kv.n_kv;
+    }
+    sh.start = c;
+  }
+  __syncthreads();
+  r.cur = sh.start;
+  return r;
+}
+
+// The CTA that holds block x of all.
+DPUF_DEV int attn_cta_of(const AttnRun& r, long long x) { return (int)(((x + 1) * r.ctas - 1) / r.total); }
+
+// Cache offset (elements) of head 0, row 0 of the page that holds position j of sequence s, or -1.
+DPUF_DEV int64_t attn_page(const AttnArgs& p, int s, int j) {
+  const int page = p.a.page_table[(size_t)s * p.a.table_stride + (j >> p.page_shift)];
+  return page < 0 || page >= p.a.kv.n_pages ? -1 : (int64_t)page * p.a.kv.page_stride;
+}
+
+}  // namespace dpuf

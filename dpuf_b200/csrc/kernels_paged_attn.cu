@@ -1,0 +1,251 @@
+// kernels_paged_attn.cu - attention of new tokens over the paged cache.
+//
+// One pass over the keys with the running maximum m and sum l of the softmax: for a block of
+// keys with scores s_j = scale * q . k_j,
+//   m' = max(m, max s_j),  p_j = exp(s_j - m'),  l' = l e^{m-m'} + sum p_j,
+//   o' = o e^{m-m'} + sum p_j v_j,  at the end out = o / l (0 where l = 0).
+// Scores are kept in units of log 2 (scale * log2(e) is folded into the product), so every
+// exponential is one ex2.  A row that has seen nothing has m = -inf and l = 0.
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "attn_plan.cuh"
+
+namespace dpuf {
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+DPUF_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a part of an item leaves behind (kRows rows of kDim floats per slot).
+template <int kRows, int kDim>
+struct AttnParts {
+  unsigned* count;  // [kAttnMaxCtas]
+  float2* ml;       // [2 kAttnMaxCtas][kRows]: maximum and sum
+  float* o;         // [2 kAttnMaxCtas][kRows][kDim]
+  static constexpr size_t bytes(int ctas) {
+    return kAttnCounterBytes + (size_t)2 * ctas * kRows * (sizeof(float2) + kDim * sizeof(float));
+  }
+  DPUF_DEV AttnParts(void* ws, int ctas) {
+    count = (unsigned*)ws;
+    ml = (float2*)((char*)ws + kAttnCounterBytes);
+    o = (float*)(ml + (size_t)2 * ctas * kRows);
+  }
+};
+
+// True in the CTA that has to join the item's parts; all of its threads see the others' parts.
+DPUF_DEV bool attn_last_part(unsigned* counter, int parts, int* flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = atomicAdd(counter, 1u) == (unsigned)(parts - 1);
+    if (last) *counter = 0;  // as the next call finds it
+    __threadfence();
+    *flag = last;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// ------------------------------------------------------------------ fp32 arithmetic, any types
+// A CTA takes 16 rows and blocks of 32 keys, both widened to fp32 in shared memory.  Thread
+// (row = tid / 16, x = tid % 16) has the scores of keys x and x + 16 and the output's dimensions
+// 4 x + 64 i of its row; a row's 16 threads are half a warp.
+constexpr int kGenRows = 16, kGenKeys = 32, kGenThreads = 256;
+
+template <typename TK, int DP>  // DP: head_dim rounded up to 64, 128 or 256
+__global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const __grid_constant__ AttnArgs p) {
+  extern __shared__ __align__(16) float sm[];
+  constexpr int kStride = DP + 4;  // rows 16 bytes apart in banks: eight rows' float4 do not collide
+  float* qs = sm;                              // [kGenRows][DP]
+  float* ks = qs + kGenRows * DP;              // [kGenKeys][kStride]
+  float* vs = ks + kGenKeys * kStride;         // [kGenKeys][kStride]
+  float* ps = vs + kGenKeys * kStride;         // [kGenRows][kGenKeys + 1]
+  __shared__ AttnShare share;
+  __shared__ int flag;
+  const int tid = threadIdx.x, row = tid >> 4, x = tid & 15;
+  const int hd = p.a.kv.head_dim;
+  AttnRun run = attn_locate<kGenRows, kGenKeys>(p, share, blockIdx.x, gridDim.x);
+  if (run.n == 0) return;
+  const AttnParts<kGenRows, DP> parts(p.a.workspace, gridDim.x);
+  AttnCursor& c = run.cur;
+  const float scale = p.a.scale * kLog2e;
+
+  for (int left = run.n; left > 0;) {
+    const int from = c.at, to = min(c.n_blk, c.at + left);
+    left -= to - from;
+    // ---- the item's rows
+    const int r0 = c.tile * kGenRows, r = r0 + row;
+    const bool live = r < c.seq.qn * p.group;
+    const int tok = live ? r / p.group : 0, head = c.head * p.group + (live ? r % p.group : 0);
+    __syncthreads();
+    for (int i = tid; i < kGenRows * DP; i += kGenThreads) {
+      const int rr = r0 + i / DP, d = i % DP;
+      float v = 0.0f;
+      if (rr < c.seq.qn * p.group && d < hd)
+        v = load_as(p.a.q, (size_t)((int64_t)(c.seq.q0 + rr / p.group) * p.a.q_stride[0] +
+                                    (int64_t)(c.head * p.group + rr % p.group) * p.a.q_stride[1] + d), p.a.dtype);
+      qs[i] = v;
+    }
+    int lo = 0, hi = 0;  // positions that this row sees
+    if (live) attn_span(p, c.seq, tok, tok, &lo, &hi);
+    int tlo, thi;        // positions that the tile sees
+    attn_span(p, c.seq, r0 / p.group, min(c.seq.qn - 1, (r0 + kGenRows - 1) / p.group), &tlo, &thi);
+    float m = -CUDART_INF_F, l = 0.0f;
+    float o[DP / 64][4] = {};
+
+    for (int b = from; b < to; b++) {
+      const int j0 = (c.blk0 + b) * kGenKeys;
+      __syncthreads();
+      for (int i = tid; i < kGenKeys * (DP / 8); i += kGenThreads) {
+        const int key = i / (DP / 8), d = i % (DP / 8) * 8, j = j0 + key;
+        float kv[8] = {}, vv[8] = {};
+        if (j >= tlo && j < thi && d < hd) {
+          const int64_t page = attn_page(p, c.s, j);
+          if (page >= 0) {
+            const int64_t at = page + (int64_t)c.head * p.a.kv.head_stride +
+                               (int64_t)(j & (p.a.kv.page_size - 1)) * p.a.kv.row_stride + d;
+            load8((const TK*)p.a.kv.k + at, kv);
+            load8((const TK*)p.a.kv.v + at, vv);
+          }
+        }
+        store8_as(ks, key * kStride + d, DPUF_TYPE_F32, kv);
+        store8_as(vs, key * kStride + d, DPUF_TYPE_F32, vv);
+      }
+      __syncthreads();
+      float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll 8
+      for (int d = 0; d < DP; d += 4) {
+        const float4 q = *(const float4*)(qs + row * DP + d);
+        const float4 a = *(const float4*)(ks + x * kStride + d), e = *(const float4*)(ks + (x + 16) * kStride + d);
+        s0 = fmaf(q.x, a.x, fmaf(q.y, a.y, fmaf(q.z, a.z, fmaf(q.w, a.w, s0))));
+        s1 = fmaf(q.x, e.x, fmaf(q.y, e.y, fmaf(q.z, e.z, fmaf(q.w, e.w, s1))));
+      }
+      s0 = j0 + x >= lo && j0 + x < hi ? s0 * scale : -CUDART_INF_F;
+      s1 = j0 + x + 16 >= lo && j0 + x + 16 < hi ? s1 * scale : -CUDART_INF_F;
+      float top = fmaxf(s0, s1);
+#pragma unroll
+      for (int i = 8; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, i));
+      const float m2 = fmaxf(m, top);
+      if (m2 != -CUDART_INF_F) {
+        const float f = ex2(m - m2);
+        const float p0 = ex2(s0 - m2), p1 = ex2(s1 - m2);
+        ps[row * (kGenKeys + 1) + x] = p0;
+        ps[row * (kGenKeys + 1) + x + 16] = p1;
+        l = fmaf(l, f, p0 + p1);  // this thread's keys only; summed over the row at the end
+        m = m2;
+#pragma unroll
+        for (int i = 0; i < DP / 64; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[i][e] *= f;
+      }
+      __syncwarp();
+      if (m != -CUDART_INF_F)
+        for (int k = 0; k < kGenKeys; k++) {
+          const float w = ps[row * (kGenKeys + 1) + k];
+#pragma unroll
+          for (int i = 0; i < DP / 64; i++) {
+            const float4 v = *(const float4*)(vs + k * kStride + 64 * i + 4 * x);
+            o[i][0] = fmaf(w, v.x, o[i][0]);
+            o[i][1] = fmaf(w, v.y, o[i][1]);
+            o[i][2] = fmaf(w, v.z, o[i][2]);
+            o[i][3] = fmaf(w, v.w, o[i][3]);
+          }
+        }
+    }
+#pragma unroll
+    for (int i = 8; i; i >>= 1) l += __shfl_xor_sync(kFull, l, i);
+
+    // ---- the whole item, or a part of it
+    const bool whole = from == 0 && to == c.n_blk;
+    bool join = false;
+    int c0 = 0, c1 = 0;
+    if (!whole) {
+      const size_t slot = 2 * (size_t)blockIdx.x + (from == 0 ? 1 : 0);
+      if (x == 0) parts.ml[slot * kGenRows + row] = make_float2(m, l);
+#pragma unroll
+      for (int i = 0; i < DP / 64; i++)
+        *(float4*)(parts.o + (slot * kGenRows + row) * DP + 64 * i + 4 * x) =
+            make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+      c0 = attn_cta_of(run, c.begin);
+      c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
+      join = attn_last_part(parts.count + c0, c1 - c0 + 1, &flag);
+      if (join) {
+        m = -CUDART_INF_F;
+        for (int cc = c0; cc <= c1; cc++)
+          m = fmaxf(m, __ldcg(&parts.ml[(2 * (size_t)cc + (cc == c0 ? 1 : 0)) * kGenRows + row]).x);
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DP / 64; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
+        if (m != -CUDART_INF_F)
+          for (int cc = c0; cc <= c1; cc++) {
+            const size_t at = (2 * (size_t)cc + (cc == c0 ? 1 : 0)) * kGenRows + row;
+            const float2 part = __ldcg(&parts.ml[at]);
+            const float f = ex2(part.x - m);
+            l = fmaf(part.y, f, l);
+#pragma unroll
+            for (int i = 0; i < DP / 64; i++) {
+              const float4 v = __ldcg((const float4*)(parts.o + at * DP + 64 * i + 4 * x));
+              o[i][0] = fmaf(v.x, f, o[i][0]);
+              o[i][1] = fmaf(v.y, f, o[i][1]);
+              o[i][2] = fmaf(v.z, f, o[i][2]);
+              o[i][3] = fmaf(v.w, f, o[i][3]);
+            }
+          }
+      }
+    }
+    if ((whole || join) && live) {
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const size_t at = ((size_t)(c.seq.q0 + tok) * p.a.n_q + head) * hd;
+#pragma unroll
+      for (int i = 0; i < DP / 64; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (64 * i + 4 * x + e < hd) store_as(p.a.out, at + 64 * i + 4 * x + e, p.a.out_dtype, o[i][e] * inv);
+    }
+    if (left > 0) attn_next_item<kGenRows, kGenKeys>(p, c);
+  }
+}
+
+template <typename TK, int DP>
+cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
+  const size_t smem = sizeof(float) * (kGenRows * DP + 2 * kGenKeys * (DP + 4) + kGenRows * (kGenKeys + 1));
+  const cudaError_t e = cudaFuncSetAttribute(paged_attention_f32_kernel<TK, DP>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  paged_attention_f32_kernel<TK, DP><<<148 * 2, kGenThreads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename TK>
+cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
+  if (p.a.kv.head_dim <= 64) return launch_f32<TK, 64>(p, s);
+  if (p.a.kv.head_dim <= 128) return launch_f32<TK, 128>(p, s);
+  return launch_f32<TK, 256>(p, s);
+}
+
+}  // namespace
+
+int64_t paged_attention_workspace() { return (int64_t)AttnParts<kGenRows, 256>::bytes(148 * 2); }
+
+cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t s) {
+  AttnArgs p;
+  p.a = a;
+  p.group = a.n_q / a.kv.n_kv;
+  p.page_shift = 31 - __builtin_clz((unsigned)a.kv.page_size);
+  p.max_kv = (int)std::min<int64_t>((int64_t)a.pages_per_seq << p.page_shift, 1 << 30);
+  if (a.kv.dtype == DPUF_TYPE_F32) return launch_f32<float>(p, s);
+  if (a.kv.dtype == DPUF_TYPE_F16) return launch_f32<__half>(p, s);
+  return launch_f32<__nv_bfloat16>(p, s);
+}
+
+}  // namespace dpuf

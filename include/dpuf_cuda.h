@@ -164,6 +164,100 @@ DPUF_EXPORT int32_t dpuf_cuda_had_asym_timed(int32_t mode, int32_t M, int32_t ro
                                              const uint64_t* tile_offsets, const uint8_t* sign_bits,
                                              int32_t n_copies, int32_t reps, float* ms_per_matmul);
 
+/* ---- serving over a paged key/value cache (no counterpart in the reference) ----
+ * The cache is two pools of pages, one for keys and one for values, that many sequences share:
+ * page p holds page_size positions of every KV head, element (p, head, row, d) at
+ * p * page_stride + head * head_stride + row * row_stride + d of k and of v.  A page table row
+ * per sequence says which page holds its positions [j * page_size, (j + 1) * page_size); an
+ * entry outside [0, n_pages) holds none.  page_size is a power of two in [8, 1024], head_dim a
+ * multiple of 8 up to 256, k, v and the strides are multiples of 16 bytes.
+ *
+ * All pointers are DEVICE pointers.  The calls enqueue on `stream` (cudaStream_t, NULL = default
+ * stream) of the current device without synchronising, allocate nothing and can be captured in
+ * a CUDA graph.  They return 0, -1 for refused arguments or -4 for a CUDA error, with the reason
+ * in dpuf_cuda_last_error().  Tables, positions and lengths stay on the device, so their values
+ * cannot be refused: every access is checked in the kernels and one that falls outside reads
+ * zeros or stores nothing. */
+enum { DPUF_TYPE_F32 = 0, DPUF_TYPE_F16 = 1, DPUF_TYPE_BF16 = 2 };
+
+typedef struct DpufPagedKv {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, row_stride; /* elements, the same for k and v */
+  int32_t dtype;                                /* DPUF_TYPE_* */
+  int32_t n_pages, n_kv, page_size, head_dim;
+  int32_t reserved;
+} DpufPagedKv;
+
+/* Rotary positions and the store of new keys and values.  Token t of sequence seq[t] stands at
+ * pos[t].  The first rotary_dim (even) dimensions of each head of q and k are turned pair by
+ * pair, (i, i + rotary_dim/2), or (2i, 2i + 1) if interleaved, with row pos[t] of the tables
+ * cos_tab and sin_tab [n_pos][rotary_dim/2]:  (a, b) -> (a cos - b sin, b cos + a sin) in fp32,
+ * rounded once.  The turned q goes to q_out [n_tokens][n_q][head_dim] (contiguous), the turned k
+ * and v go to the cache.  dtype is that of q, k and v, out_dtype that of q_out.  A token with
+ * pos < 0 is padding (q_out gets zeros, nothing is stored); one with pos >= n_pos has no table
+ * row (q_out gets NaN, nothing is stored); one whose page is not held is not stored.  Tokens of
+ * one call that share a position race. */
+typedef struct DpufRopeAppendArgs {
+  DpufPagedKv kv;
+  const int32_t* page_table; /* [n_seqs][table_stride], pages_per_seq entries used */
+  int64_t table_stride;
+  const void *q, *k, *v;     /* element (t, head, d) at t * stride[0] + head * stride[1] + d */
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  void* q_out;
+  const float *cos_tab, *sin_tab;
+  const int32_t *seq, *pos;  /* [n_tokens] */
+  int32_t n_seqs, pages_per_seq, n_tokens, n_q, rotary_dim, n_pos, interleaved, dtype, out_dtype;
+  int32_t reserved;
+} DpufRopeAppendArgs;
+DPUF_EXPORT int32_t dpuf_cuda_rope_append(const DpufRopeAppendArgs* args, void* stream);
+
+/* Attention of new tokens over the paged cache.  Sequence s has the new tokens q_start[s] ..
+ * q_start[s+1] (q_start[0] = 0, q_start[n_seqs] = n_tokens), which are the last of its
+ * kv_len[s] positions and are in the cache already.  The token at position p sees the positions
+ * j <= p (all kv_len[s] if causal is 0), and with window > 0 only j > p - window;
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,
+ * zeros for a token that sees nothing.  Query head h reads KV head h / (n_q / n_kv).  max_q (at
+ * least the largest q_start[s+1] - q_start[s]; rows beyond it are not written) chooses the
+ * kernel and the grid.  dtype is that of q and is float32 or the cache's, out_dtype that of out
+ * [n_tokens][n_q][head_dim] (contiguous) and is dtype or float32.  Positions that no token of a
+ * sequence sees are never used, whatever stands there; a value that is not finite at a position
+ * below kv_len[s] may reach every row of that sequence.
+ * workspace: dpuf_cuda_paged_attention_workspace() bytes, 16-byte aligned, all zero before its
+ * first use (each call leaves its counters at zero); calls that share one must not overlap. */
+typedef struct DpufPagedAttentionArgs {
+  DpufPagedKv kv;
+  const int32_t* page_table; /* [n_seqs][table_stride], pages_per_seq entries used */
+  int64_t table_stride;
+  const void* q;             /* element (t, head, d) at t * stride[0] + head * stride[1] + d */
+  int64_t q_stride[2];
+  void* out;
+  const int32_t *q_start, *kv_len;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t n_seqs, pages_per_seq, n_tokens, n_q, max_q, causal, window, dtype, out_dtype;
+  float scale;
+} DpufPagedAttentionArgs;
+DPUF_EXPORT int64_t dpuf_cuda_paged_attention_workspace(void);
+DPUF_EXPORT int32_t dpuf_cuda_paged_attention(const DpufPagedAttentionArgs* args, void* stream);
+
+/* Sampling on the device: one token per row of logits [rows][vocab] (row stride row_stride
+ * elements, vocab <= 2^20, dtype DPUF_TYPE_*) from the given uniforms u[rows] in [0, 1).
+ * temperature, top_k, top_p, min_p are per-row arrays; a null one means 1, 0, 1, 0.
+ *   w_i = exp((l_i - max l) / temperature) in fp32 (0 for NaN)
+ *   kept: of the entries ordered by (l down, index up) the first top_k (all if < 1); of these
+ *   the shortest prefix holding top_p of their weight (all if >= 1, never none); of these the
+ *   ones with w_i >= min(min_p, 1)
+ *   id = the first kept index, in index order, whose running weight exceeds u * (kept weight)
+ *   prob = w_id / (kept weight)
+ * With temperature <= 0 the id is the first index of the maximum, with prob 1.  A row with no
+ * entry above -inf gives id -1, prob 0.  Sums are exact in fixed point (weights in units of
+ * 2^-43), so ids do not depend on the order of additions.  probs may be null. */
+DPUF_EXPORT int32_t dpuf_cuda_sample_rows(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
+                                          int32_t vocab, const float* u, const float* temperature,
+                                          const int32_t* top_k, const float* top_p, const float* min_p,
+                                          int32_t* ids, float* probs, void* stream);
+
 /* Builds or loads the glibc expf exception table; returns its entry count (host only). */
 DPUF_EXPORT int64_t dpuf_cuda_prepare_expf_table(void);
 
