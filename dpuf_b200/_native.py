@@ -43,6 +43,7 @@ CUDA_SOURCES = [
     "sampling.cu",
     "kernels_rope.cu",
     "kernels_paged_attn.cu",
+    "kernels_paged_attn_tc.cu",
     "kernels_sample.cu",
     "ops_serving.cu",
 ]

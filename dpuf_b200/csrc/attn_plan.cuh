@@ -17,7 +17,7 @@
 namespace dpuf {
 
 constexpr int kAttnMaxCtas = 148 * 4;
-constexpr int kAttnCounterBytes = (kAttnMaxCtas * 4 + 255) & ~255;
+constexpr int kAttnCounterBytes = (kAttnMaxCtas * 8 + 255) & ~255;
 
 struct AttnArgs {
   DpufPagedAttentionArgs a;

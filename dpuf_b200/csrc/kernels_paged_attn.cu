@@ -10,7 +10,7 @@
 
 #include <algorithm>
 
-#include "attn_plan.cuh"
+#include "attn_parts.cuh"
 
 namespace dpuf {
 
@@ -24,32 +24,11 @@ DPUF_DEV float ex2(float x) {
   return y;
 }
 
-// What a part of an item leaves behind (kRows rows of kDim floats per slot).
-template <int kRows, int kDim>
-struct AttnParts {
-  unsigned* count;  // [kAttnMaxCtas]
-  float2* ml;       // [2 kAttnMaxCtas][kRows]: maximum and sum
-  float* o;         // [2 kAttnMaxCtas][kRows][kDim]
-  static constexpr size_t bytes(int ctas) {
-    return kAttnCounterBytes + (size_t)2 * ctas * kRows * (sizeof(float2) + kDim * sizeof(float));
-  }
-  DPUF_DEV AttnParts(void* ws, int ctas) {
-    count = (unsigned*)ws;
-    ml = (float2*)((char*)ws + kAttnCounterBytes);
-    o = (float*)(ml + (size_t)2 * ctas * kRows);
-  }
-};
-
 // True in the CTA that has to join the item's parts; all of its threads see the others' parts.
 DPUF_DEV bool attn_last_part(unsigned* counter, int parts, int* flag) {
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const bool last = atomicAdd(counter, 1u) == (unsigned)(parts - 1);
-    if (last) *counter = 0;  // as the next call finds it
-    __threadfence();
-    *flag = last;
-  }
+  if (threadIdx.x == 0) *flag = attn_arrive(counter, parts);
   __syncthreads();
   return *flag != 0;
 }
@@ -176,7 +155,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
             make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
       c0 = attn_cta_of(run, c.begin);
       c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
-      join = attn_last_part(parts.count + c0, c1 - c0 + 1, &flag);
+      join = attn_last_part(parts.count + 2 * c0, c1 - c0 + 1, &flag);
       if (join) {
         m = -CUDART_INF_F;
         for (int cc = c0; cc <= c1; cc++)
@@ -218,11 +197,10 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
 
 template <typename TK, int DP>
 cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
-  const size_t smem = sizeof(float) * (kGenRows * DP + 2 * kGenKeys * (DP + 4) + kGenRows * (kGenKeys + 1));
-  const cudaError_t e = cudaFuncSetAttribute(paged_attention_f32_kernel<TK, DP>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  constexpr size_t smem = sizeof(float) * (kGenRows * DP + 2 * kGenKeys * (DP + 4) + kGenRows * (kGenKeys + 1));
+  const cudaError_t e = smem_limit_once<paged_attention_f32_kernel<TK, DP>>((int)smem);
   if (e != cudaSuccess) return e;
-  paged_attention_f32_kernel<TK, DP><<<148 * 2, kGenThreads, smem, s>>>(p);
+  paged_attention_f32_kernel<TK, DP><<<kAttnSms * 2, kGenThreads, smem, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -235,7 +213,18 @@ cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
 
 }  // namespace
 
-int64_t paged_attention_workspace() { return (int64_t)AttnParts<kGenRows, 256>::bytes(148 * 2); }
+int64_t paged_attention_workspace() {
+  return (int64_t)std::max(AttnParts<kGenRows, 256>::bytes(kAttnSms * 2), paged_attention_tc_workspace());
+}
+
+cudaError_t paged_attention_status(void* workspace, bool* gave_up, cudaStream_t s) {
+  int word = 0;
+  cudaError_t e = cudaMemcpyAsync(&word, attn_error(workspace), sizeof(word), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  *gave_up = word != 0;
+  if (e == cudaSuccess && word) e = cudaMemsetAsync(workspace, 0, kAttnHeader + kAttnCounterBytes, s);
+  return e;
+}
 
 cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t s) {
   AttnArgs p;
@@ -243,6 +232,8 @@ cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t
   p.group = a.n_q / a.kv.n_kv;
   p.page_shift = 31 - __builtin_clz((unsigned)a.kv.page_size);
   p.max_kv = (int)std::min<int64_t>((int64_t)a.pages_per_seq << p.page_shift, 1 << 30);
+  if (a.dtype == a.kv.dtype && a.dtype != DPUF_TYPE_F32 && a.kv.head_dim <= 128 && a.max_q * p.group > 16)
+    return launch_paged_attention_tc(p, s);
   if (a.kv.dtype == DPUF_TYPE_F32) return launch_f32<float>(p, s);
   if (a.kv.dtype == DPUF_TYPE_F16) return launch_f32<__half>(p, s);
   return launch_f32<__nv_bfloat16>(p, s);

@@ -1,0 +1,632 @@
+// kernels_paged_attn_tc.cu - attention of chunks of new tokens over the paged cache on the
+// 5th-generation tensor cores (tcgen05, TMEM), 16-bit queries and cache, head_dim <= 128.
+//
+// An item is 256 rows of one sequence and KV head (two tiles of 128), walked in blocks of 128
+// keys; per tile and block S = Q K^T (M = 128, N = 128) into TMEM, the softmax's weights P from S
+// with the running maximum and sum (kernels_paged_attn.cu has the formulas), O += P V with P read
+// from TMEM.  Two tiles share the keys and values, and while one's softmax runs on the CUDA cores
+// the other's products run on the tensor cores.
+//
+//   warps 0..3, 4..7  softmax of tile 0, 1: a thread has one row.  It reads its 128 scores, writes
+//                     P (rounded to the cache's type; the sum keeps the unrounded weights) over
+//                     them, and scales O in TMEM only when its row's maximum has grown by more
+//                     than 2^8 since the last time (weights are then at most 2^8, which both types
+//                     hold with their full precision; the division by the sum at the end makes up
+//                     for it), which after the first blocks is rare.
+//   warp 8            TMA: 64-column boxes of a page's rows (128-byte swizzle) into a ring of key
+//                     and value blocks; a page that is not held, or that no row sees, is a box
+//                     outside the tensor and arrives as zeros.
+//   warp 9            issues the MMAs of whichever tile is ready, each tile's products in turn;
+//                     zeroes the rows of a value block that no row of the item sees (stale cache
+//                     contents may be infinite or NaN, and 0 times those is NaN; scores of such
+//                     keys are replaced, not multiplied).
+//
+// TMEM: S0, S1 (128 columns each; P in the first 64), O0, O1.  A tile's next S may only be
+// written once its P has been read, so the QK of block b + 1 waits for the PV of block b.
+//
+// Every wait is bounded: one that gives up sets the workspace's error word and the CTA's abort
+// flag, all roles stop, copies in flight are waited for (bounded) and TMEM is freed.
+#include <cuda.h>
+#include <math_constants.h>
+
+#include "attn_plan.cuh"
+#include "attn_parts.cuh"
+
+namespace dpuf {
+
+namespace {
+
+constexpr int kTile = 128;            // rows of a tile, keys of a block
+constexpr int kItemRows = 2 * kTile;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 320;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+DPUF_DEV uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// Shared-memory descriptor of a 128-byte swizzled operand: K-major (lbo unused, sbo between
+// groups of 8 rows), or MN-major (lbo between runs of 64 columns, sbo between groups of 8 rows).
+DPUF_DEV uint64_t sw128_desc(const void* p, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((su32(p) >> 4) & 0x3FFF) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16: D fp32, A and B of one type (0 f16, 1 bf16), A K-major, B K- or MN-major, M = 128.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn) {
+  const uint32_t t = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kTile >> 4) << 24);
+}
+
+DPUF_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
+      : "memory");
+}
+DPUF_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((int)acc)
+      : "memory");
+}
+DPUF_DEV void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar))
+               : "memory");
+}
+#define DPUF_R32(v)                                                                                             \
+  "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),   \
+      "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),    \
+      "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),   \
+      "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+#define DPUF_I32(v)                                                                                             \
+  "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), \
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),           \
+      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),           \
+      "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+// 32 columns of the warp's 32 lanes; the values are there after tmem_wait_ld.
+DPUF_DEV void tmem_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : DPUF_R32(v)
+      : "r"(addr));
+}
+DPUF_DEV void tmem_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::DPUF_I32(v),
+      "r"(addr)
+      : "memory");
+}
+// 8 columns, there on return.
+DPUF_DEV void tmem_ld8(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+      : "r"(addr)
+      : "memory");
+}
+DPUF_DEV void tmem_st8(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
+               : "memory");
+}
+DPUF_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+DPUF_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+DPUF_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+DPUF_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+DPUF_DEV unsigned long long gtimer() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+DPUF_DEV void bar_init(uint64_t* bar, int n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(bar)), "r"(n) : "memory");
+}
+DPUF_DEV void bar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(bar)) : "memory");
+}
+DPUF_DEV bool bar_try(uint64_t* bar, unsigned par) {
+  unsigned ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(su32(bar)), "r"(par)
+               : "memory");
+  return ok != 0;
+}
+DPUF_DEV bool bar_test(uint64_t* bar, unsigned par) {
+  unsigned ok;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(su32(bar)), "r"(par)
+               : "memory");
+  return ok != 0;
+}
+
+struct Give {  // where a wait that gives up says so
+  volatile int* abort;
+  int* err;
+};
+// Waits of a whole warp: true once the phase is complete, false (for all lanes) after giving up.
+DPUF_DEV bool warp_wait(uint64_t* bar, unsigned par, const Give& g) {
+  bool ok = bar_try(bar, par);
+  if (!ok) {
+    const unsigned long long t0 = gtimer();
+    for (int it = 1; !ok; it++) {
+      ok = bar_try(bar, par);
+      if (!ok && (it & 15) == 0 && (*g.abort || gtimer() - t0 > kWaitNs)) {
+        *g.abort = 1;
+        atomicCAS(g.err, 0, 1);
+        break;
+      }
+    }
+  }
+  return __all_sync(kFull, ok);
+}
+
+DPUF_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+DPUF_DEV uint32_t pack2(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *(const uint32_t*)&h;
+}
+DPUF_DEV uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *(const uint32_t*)&h;
+}
+
+template <int DP>
+struct TileLay {  // shared memory, from a 1,024-byte boundary
+  static constexpr int stages = DP == 128 ? 2 : 4;
+  static constexpr int block = kTile * DP * 2;  // 64-column runs of [128][128 bytes]
+  static constexpr int q = 0;                   // [2][block]
+  static constexpr int k = q + 2 * block;       // [stages][block]
+  static constexpr int v = k + stages * block;  // [stages][block]
+  static constexpr int bytes = v + stages * block + 1024;
+};
+constexpr int kRun = kTile * 128;  // bytes of a 64-column run
+
+struct TileArgs {
+  AttnArgs p;
+  CUtensorMap k_map, v_map;  // (dim, row, head, page), boxes of 64 x min(page_size, 128)
+};
+
+// Positions that an item's rows [r0, r0 + rows) see between them.
+DPUF_DEV void item_span(const AttnArgs& p, const AttnSeq& q, int tile, int* lo, int* hi) {
+  attn_span(p, q, tile * kItemRows / p.group, min(q.qn - 1, (tile * kItemRows + kItemRows - 1) / p.group), lo, hi);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const __grid_constant__ TileArgs args) {
+  using Lay = TileLay<DP>;
+  constexpr int S = Lay::stages;
+  extern __shared__ unsigned char raw[];
+  __shared__ __align__(8) uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S];
+  __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+  __shared__ AttnShare share;
+  __shared__ uint32_t tmem_sh;
+  __shared__ int abort_sh, flag_sh[2];
+  unsigned char* const sm = raw + ((1024 - (su32(raw) & 1023)) & 1023);
+  const AttnArgs& p = args.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const AttnParts<kItemRows, DP> parts(p.a.workspace, gridDim.x);
+  const Give give{&abort_sh, attn_error(p.a.workspace)};
+
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_sh)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < S; i++) {
+      bar_init(&k_full[i], 1);
+      bar_init(&k_empty[i], 1);
+      bar_init(&v_full[i], 1);
+      bar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      bar_init(&q_full[i], kTile);
+      bar_init(&s_full[i], 1);
+      bar_init(&p_full[i], kTile);
+      bar_init(&pv_done[i], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    abort_sh = 0;
+  }
+  fence_before();
+  AttnRun run = attn_locate<kItemRows, kTile>(p, share, blockIdx.x, gridDim.x);
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_sh;
+  AttnCursor& c = run.cur;
+
+  if (warp == kLoadWarp) {
+    // ================================================================ TMA
+    const int box = min(p.a.kv.page_size, kTile), boxes = kTile / box;
+    unsigned it = 0;  // blocks requested so far
+    bool ok = true;
+    for (int left = run.n; ok && left > 0;) {
+      const int from = c.at, to = min(c.n_blk, c.at + left);
+      left -= to - from;
+      int lo, hi;
+      item_span(p, c.seq, c.tile, &lo, &hi);
+      auto page_of = [&](int b) {  // of this lane's box
+        const int j = (c.blk0 + b) * kTile + lane * box;
+        int page = p.a.kv.n_pages;  // outside the tensor
+        if (lane < boxes && j < hi && j + box > lo) {
+          page = p.a.page_table[(size_t)c.s * p.a.table_stride + (j >> p.page_shift)];
+          if (page < 0 || page > p.a.kv.n_pages) page = p.a.kv.n_pages;
+        }
+        return page;
+      };
+      int page = page_of(from);
+      for (int b = from; ok && b < to; b++, it++) {
+        const int next = b + 1 < to ? page_of(b + 1) : 0;
+        const int slot = it % S;
+        const unsigned par = (it / S & 1) ^ 1;
+        const int row = ((c.blk0 + b) * kTile + lane * box) & (p.a.kv.page_size - 1);
+        auto copy = [&](const CUtensorMap* map, uint64_t* full, unsigned char* dst) {
+          if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(full)), "r"(Lay::block)
+                         : "memory");
+          __syncwarp();
+          if (lane < boxes)
+#pragma unroll
+            for (int h = 0; h < DP / 64; h++)
+              asm volatile(
+                  "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+                  "%3, %4, %5}], [%6];" ::"r"(su32(dst + h * kRun + lane * box * 128)),
+                  "l"(map), "r"(h * 64), "r"(row), "r"(c.head), "r"(page), "r"(su32(full))
+                  : "memory");
+        };
+        if (!(ok = warp_wait(&k_empty[slot], par, give))) break;
+        copy(&args.k_map, &k_full[slot], sm + Lay::k + slot * Lay::block);
+        if (!(ok = warp_wait(&v_empty[slot], par, give))) {
+          it++;
+          break;
+        }
+        copy(&args.v_map, &v_full[slot], sm + Lay::v + slot * Lay::block);
+        page = next;
+      }
+      if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+    }
+    if (!ok)  // nothing in flight at exit (waits of at most 2 s each; a value block may be missing)
+      for (unsigned i = it > S ? it - S : 0; i < it; i++) {
+        const unsigned long long t0 = gtimer();
+        while (!bar_try(&k_full[i % S], i / S & 1) && gtimer() - t0 < kWaitNs) {}
+        const unsigned long long t1 = gtimer();
+        while (!bar_try(&v_full[i % S], i / S & 1) && gtimer() - t1 < kWaitNs / 100) {}
+      }
+  } else if (warp == kMmaWarp) {
+    // ================================================================ MMA
+    constexpr uint32_t kIdQk = idesc_f16<T>(kTile, 0), kIdPv = idesc_f16<T>(DP, 1);
+    unsigned base = 0;                     // blocks of earlier items
+    unsigned items[2] = {0, 0};            // items and blocks of each tile so far
+    unsigned blocks[2] = {0, 0};
+    bool ok = true;
+    for (int left = run.n; ok && left > 0;) {
+      const int from = c.at, to = min(c.n_blk, c.at + left), n = to - from;
+      left -= n;
+      int lo, hi;
+      item_span(p, c.seq, c.tile, &lo, &hi);
+      const int tiles = c.seq.qn * p.group - c.tile * kItemRows > kTile ? 2 : 1;
+      int qk[2] = {0, 0}, pv[2] = {0, 0}, cleaned = -1;
+      unsigned long long t0 = 0;
+      for (int idle = 0;;) {
+        bool moved = false;
+        for (int i = 0; i < tiles; i++) {
+          if (pv[i] == n) continue;
+          const bool want_qk = qk[i] == pv[i];
+          const int b = want_qk ? qk[i] : pv[i];
+          const unsigned g = base + b;
+          const int slot = g % S;
+          const unsigned par = g / S & 1;
+          if (want_qk) {
+            bool ready = bar_test(&k_full[slot], par);
+            if (b == 0) ready = ready && bar_test(&q_full[i], items[i] & 1);
+            if (blocks[i] > 0) ready = ready && bar_test(&pv_done[i], (blocks[i] - 1) & 1);
+            if (!__all_sync(kFull, ready)) continue;
+            if (lane == 0) {
+              fence_after();
+              const uint64_t da = sw128_desc(sm + Lay::q + i * Lay::block, 16, 1024);
+              const uint64_t db = sw128_desc(sm + Lay::k + slot * Lay::block, 16, 1024);
+#pragma unroll
+              for (int s = 0; s < DP / 16; s++) {  // 16 columns = 32 bytes a step
+                const uint64_t o = (uint64_t)((s / 4) * (kRun >> 4) + (s % 4) * 2);
+                mma_ss(tmem + i * kTile, da + o, db + o, kIdQk, s > 0);
+              }
+              mma_commit(&s_full[i]);
+            }
+            qk[i]++;
+            if (tiles == 1 || qk[i ^ 1] > b) {
+              if (lane == 0) mma_commit(&k_empty[slot]);
+            }
+          } else {
+            bool ready = bar_test(&v_full[slot], par) && bar_test(&p_full[i], blocks[i] & 1);
+            if (!__all_sync(kFull, ready)) continue;
+            if (cleaned < b) {  // once per value block
+              cleaned = b;
+              const int j0 = (c.blk0 + from + b) * kTile;
+              const int z0 = max(lo - j0, 0), z1 = min(hi - j0, kTile);  // rows to keep
+              if (z0 > 0 || z1 < kTile) {
+                unsigned char* v = sm + Lay::v + slot * Lay::block;
+                for (int r = lane >> 3; r < kTile; r += 4)
+                  if (r < z0 || r >= z1)
+#pragma unroll
+                    for (int h = 0; h < DP / 64; h++)
+                      *(uint4*)(v + h * kRun + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+              }
+            }
+            if (lane == 0) {
+              fence_after();
+              const uint64_t db = sw128_desc(sm + Lay::v + slot * Lay::block, kRun, 1024);
+#pragma unroll
+              for (int s = 0; s < kTile / 16; s++)  // 16 keys = 2,048 bytes of V, 8 columns of P a step
+                mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + s * 8, db + (uint64_t)(s * 128), kIdPv,
+                       b > 0 || s > 0);
+              mma_commit(&pv_done[i]);
+            }
+            pv[i]++;
+            blocks[i]++;
+            if (tiles == 1 || pv[i ^ 1] > b) {
+              if (lane == 0) mma_commit(&v_empty[slot]);
+            }
+          }
+          moved = true;
+        }
+        if (pv[0] == n && (tiles == 1 || pv[1] == n)) break;
+        if (moved) {
+          idle = 0;
+        } else if (++idle == 64) {
+          t0 = gtimer();
+        } else if (idle > 64 && (idle & 63) == 0) {
+          bool late = gtimer() - t0 > kWaitNs;
+          if (late) {
+            *give.abort = 1;
+            atomicCAS(give.err, 0, 1);
+          }
+          if (__any_sync(kFull, late || *give.abort)) {
+            ok = false;
+            break;
+          }
+        }
+      }
+      for (int i = 0; i < tiles; i++) items[i]++;
+      base += n;
+      if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+    }
+  } else {
+    // ================================================================ softmax: tile w, this thread's row
+    const int w = warp >> 2, t = tid & (kTile - 1);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + w * kTile + lanes, tO = tmem + 2 * kTile + w * kTile + lanes;
+    // not 0, so that a hidden score (-inf) stays one
+    const float sl = fmaxf(fabsf(p.a.scale) * 1.44269504088896341f, 1e-37f);
+    const uint32_t flip = p.a.scale < 0.0f ? 0x80008000u : 0u;  // the sign goes with Q
+    const int hd = p.a.kv.head_dim;
+    unsigned blocks = 0;
+    bool ok = true;
+    auto wg_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); };
+    for (int left = run.n; ok && left > 0;) {
+      const int from = c.at, to = min(c.n_blk, c.at + left), n = to - from;
+      left -= n;
+      const int total = c.seq.qn * p.group, r0 = c.tile * kItemRows + w * kTile;
+      if (w == 1 && r0 >= total) {  // one tile only
+        if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+        continue;
+      }
+      // ---- this tile's queries (the earlier item's products are complete: its last scores were)
+      unsigned char* qs = sm + Lay::q + w * Lay::block;
+      for (int i = t; i < kTile * (DP / 8); i += kTile) {
+        const int r = i / (DP / 8), ch = i % (DP / 8), rr = r0 + r;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (rr < total && ch * 8 < hd) {
+          x = *(const uint4*)((const T*)p.a.q + (int64_t)(c.seq.q0 + rr / p.group) * p.a.q_stride[0] +
+                              (int64_t)(c.head * p.group + rr % p.group) * p.a.q_stride[1] + ch * 8);
+          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+        }
+        *(uint4*)(qs + (ch >> 3) * kRun + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(&q_full[w]);
+      const int r = r0 + t;
+      const bool live = r < total;
+      const int tok = live ? r / p.group : 0, head = c.head * p.group + (live ? r % p.group : 0);
+      int lo = 0, hi = 0;
+      if (live) attn_span(p, c.seq, tok, tok, &lo, &hi);
+      float m = -CUDART_INF_F, l = 0.0f;  // m: the maximum that the weights refer to
+      for (int b = 0; b < n; b++, blocks++) {
+        const int j0 = (c.blk0 + from + b) * kTile;
+        if (!(ok = warp_wait(&s_full[w], blocks & 1, give))) break;
+        fence_after();
+        uint32_t s[kTile];
+#pragma unroll
+        for (int i = 0; i < 4; i++) tmem_ld32(tS + 32 * i, s + 32 * i);
+        tmem_wait_ld();
+        if (!__all_sync(kFull, lo <= j0 && j0 + kTile <= hi)) {
+          const int a = lo - j0, e = hi - j0;
+#pragma unroll
+          for (int i = 0; i < kTile; i++)
+            if (i < a || i >= e) s[i] = 0xFF800000u;  // -inf
+        }
+        float t4[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) t4[i] = __uint_as_float(s[i]);
+#pragma unroll
+        for (int i = 4; i < kTile; i++) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(s[i]));
+        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+        const bool grow = b == 0 || m == -CUDART_INF_F ? top > m : (top - m) * sl > 8.0f;
+        if (__any_sync(kFull, grow)) {
+          const float m2 = grow ? top : m;
+          const float f = !grow ? 1.0f : m == -CUDART_INF_F ? 0.0f : ex2((m - m2) * sl);
+          l *= f;
+          m = m2;
+          if (b > 0) {
+#pragma unroll 1
+            for (int i = 0; i < DP / 8; i++) {  // few columns at a time: the scores hold the registers
+              uint32_t o[8];
+              tmem_ld8(tO + 8 * i, o);
+#pragma unroll
+              for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st8(tO + 8 * i, o);
+            }
+          }
+        }
+        const float ref = m == -CUDART_INF_F ? 0.0f : m * sl;
+        float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kTile; i += 2) {
+          const float a = ex2(__fmaf_rn(__uint_as_float(s[i]), sl, -ref));
+          const float e = ex2(__fmaf_rn(__uint_as_float(s[i + 1]), sl, -ref));
+          l4[i / 2 & 3] += a + e;
+          s[i / 2] = pack2(a, e, T());
+        }
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        tmem_st32(tS, s);
+        tmem_st32(tS + 32, s + 32);
+        tmem_wait_st();
+        fence_before();
+        bar_arrive(&p_full[w]);
+      }
+      if (!ok || !(ok = warp_wait(&pv_done[w], (blocks - 1) & 1, give))) break;
+      fence_after();
+
+      // ---- the whole item, or a part of it
+      const bool whole = from == 0 && to == c.n_blk;
+      bool join = false;
+      int c0 = 0, c1 = 0;
+      if (!whole) {
+        const size_t slot = 2 * (size_t)blockIdx.x + (from == 0 ? 1 : 0);
+        const int pr = w * kTile + t;
+        parts.ml[slot * kItemRows + pr] = make_float2(m * sl, l);
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+          uint32_t o[32];
+          tmem_ld32(tO + 32 * i, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e++)  // [dim][row]: a warp's rows are adjacent
+            parts.o[(slot * DP + 32 * i + e) * kItemRows + pr] = __uint_as_float(o[e]);
+        }
+        c0 = attn_cta_of(run, c.begin);
+        c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
+        __threadfence();
+        wg_sync();
+        if (t == 0) flag_sh[w] = attn_arrive(parts.count + 2 * c0 + w, c1 - c0 + 1);
+        wg_sync();
+        join = flag_sh[w] != 0;
+        if (join) {
+          float top = -CUDART_INF_F;
+          for (int cc = c0; cc <= c1; cc++)
+            top = fmaxf(top, __ldcg(&parts.ml[(2 * (size_t)cc + (cc == c0)) * kItemRows + pr]).x);
+          m = top;
+          l = 0.0f;
+          for (int cc = c0; cc <= c1; cc++) {
+            const float2 x = __ldcg(&parts.ml[(2 * (size_t)cc + (cc == c0)) * kItemRows + pr]);
+            l = __fmaf_rn(x.y, x.x == -CUDART_INF_F ? 0.0f : ex2(x.x - top), l);
+          }
+        }
+      }
+      if (whole || join) {
+        const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+        const size_t at = ((size_t)(c.seq.q0 + tok) * p.a.n_q + head) * hd;
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+          uint32_t o[32];
+          if (whole) {
+            tmem_ld32(tO + 32 * i, o);
+            tmem_wait_ld();
+          } else {
+            const int pr = w * kTile + t;
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = 0;
+            for (int cc = c0; cc <= c1; cc++) {
+              const size_t slot = 2 * (size_t)cc + (cc == c0);
+              const float x = __ldcg(&parts.ml[slot * kItemRows + pr]).x;
+              const float f = x == -CUDART_INF_F ? 0.0f : ex2(x - m);
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                o[e] = __float_as_uint(__fmaf_rn(__ldcg(&parts.o[(slot * DP + 32 * i + e) * kItemRows + pr]), f,
+                                                 __uint_as_float(o[e])));
+            }
+          }
+          if (live)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+              if (32 * i + 8 * g < hd) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = __uint_as_float(o[8 * g + e]) * inv;
+                store8_as(p.a.out, at + 32 * i + 8 * g, p.a.out_dtype, x);
+              }
+        }
+      }
+      fence_before();  // O is read: the next item's products may overwrite it once its P arrives
+      if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return (EncodeFn)f;
+  }();
+  return fn;
+}
+
+bool encode(CUtensorMap* map, const DpufPagedKv& kv, void* base) {
+  const cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_kv,
+                              (cuuint64_t)kv.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)kv.row_stride * 2, (cuuint64_t)kv.head_stride * 2,
+                                 (cuuint64_t)kv.page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(kv.page_size, kTile), 1, 1}, one[4] = {1, 1, 1, 1};
+  return encoder()(map, kv.dtype == DPUF_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                   4, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP>
+cudaError_t launch(const TileArgs& a, cudaStream_t s) {
+  const cudaError_t e = smem_limit_once<paged_attention_tc_kernel<T, DP>>(TileLay<DP>::bytes);
+  if (e != cudaSuccess) return e;
+  paged_attention_tc_kernel<T, DP><<<kAttnSms, kThreads, TileLay<DP>::bytes, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t paged_attention_tc_workspace() { return AttnParts<kItemRows, 128>::bytes(kAttnSms); }
+
+cudaError_t launch_paged_attention_tc(const AttnArgs& p, cudaStream_t s) {
+  if (!encoder()) return cudaErrorNotSupported;
+  TileArgs a;
+  a.p = p;
+  if (!encode(&a.k_map, p.a.kv, p.a.kv.k) || !encode(&a.v_map, p.a.kv, p.a.kv.v)) return cudaErrorInvalidValue;
+  const bool small = p.a.kv.head_dim <= 64;
+  if (p.a.kv.dtype == DPUF_TYPE_F16) return small ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+  return small ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace dpuf

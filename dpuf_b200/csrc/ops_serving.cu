@@ -109,6 +109,17 @@ DPUF_EXPORT int32_t dpuf_cuda_paged_attention(const DpufPagedAttentionArgs* args
   return finish(me, launch_paged_attention(a, (cudaStream_t)stream));
 }
 
+DPUF_EXPORT int32_t dpuf_cuda_paged_attention_status(void* workspace, void* stream) {
+  const char* me = "dpuf_cuda_paged_attention_status";
+  set_error("");
+  if (!workspace) return refuse(me, "null workspace");
+  bool gave_up = false;
+  const int32_t rc = finish(me, paged_attention_status(workspace, &gave_up, (cudaStream_t)stream));
+  if (rc != 0 || !gave_up) return rc;
+  set_error(std::string(me) + ": a bounded wait in an attention kernel gave up");
+  return -6;
+}
+
 DPUF_EXPORT int32_t dpuf_cuda_sample_rows(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
                                           int32_t vocab, const float* u, const float* temperature,
                                           const int32_t* top_k, const float* top_p, const float* min_p,

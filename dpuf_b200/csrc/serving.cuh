@@ -87,6 +87,7 @@ DPUF_DEV void store8_as(void* p, size_t i, int dtype, const float (&v)[8]) {
 cudaError_t launch_rope_append(const DpufRopeAppendArgs& a, bool vectors, cudaStream_t s);
 cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t s);
 int64_t paged_attention_workspace();
+cudaError_t paged_attention_status(void* workspace, bool* gave_up, cudaStream_t s);
 cudaError_t launch_sample_rows(const void* logits, int dtype, int64_t row_stride, int rows, int vocab, const float* u,
                                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                                int32_t* ids, float* probs, cudaStream_t s);

@@ -47,6 +47,8 @@ def _lib():
         lib.dpuf_cuda_paged_attention.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
         lib.dpuf_cuda_paged_attention_workspace.restype = ctypes.c_int64
         lib.dpuf_cuda_paged_attention_workspace.argtypes = []
+        lib.dpuf_cuda_paged_attention_status.restype = ctypes.c_int32
+        lib.dpuf_cuda_paged_attention_status.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         lib.dpuf_cuda_sample_rows.restype = ctypes.c_int32
         lib.dpuf_cuda_sample_rows.argtypes = ([ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int32,
                                                ctypes.c_int32] + [ctypes.c_void_p] * 8)
@@ -271,6 +273,13 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
         _CODE[out.dtype], hd ** -0.5 if scale is None else scale)
     _call(_lib().dpuf_cuda_paged_attention, dev, args)
     return out
+
+
+def attention_check(device: int | None = None) -> None:
+    """Waits for the current stream and raises RuntimeError if a bounded wait inside one of its
+    `paged_attention` calls gave up since the last check (that call's output is undefined)."""
+    dev = torch.cuda.current_device() if device is None else device
+    _call(_lib().dpuf_cuda_paged_attention_status, dev, _workspace(dev).data_ptr())
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None,

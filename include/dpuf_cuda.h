@@ -240,6 +240,10 @@ typedef struct DpufPagedAttentionArgs {
 } DpufPagedAttentionArgs;
 DPUF_EXPORT int64_t dpuf_cuda_paged_attention_workspace(void);
 DPUF_EXPORT int32_t dpuf_cuda_paged_attention(const DpufPagedAttentionArgs* args, void* stream);
+/* Waits for `stream` and says whether every wait inside the kernels that used the workspace was
+ * met: 0, or -6 if one gave up (2 s; that call's output is undefined; the workspace is then made
+ * ready for use again), -1 or -4 as above. */
+DPUF_EXPORT int32_t dpuf_cuda_paged_attention_status(void* workspace, void* stream);
 
 /* Sampling on the device: one token per row of logits [rows][vocab] (row stride row_stride
  * elements, vocab <= 2^20, dtype DPUF_TYPE_*) from the given uniforms u[rows] in [0, 1).

@@ -200,6 +200,7 @@ def run_attention(types, heads, hd, page, q_lens, kv_lens, causal=True, window=0
     kv_len = torch.tensor(kv_lens, dtype=INT, device="cuda")
     got = serving.paged_attention(cache, table, q, q_start, kv_len, max(max(q_lens), 1), scale, causal, window, out)
     want, bound = attention64(cache, table, q, start, lens, hd ** -0.5 if scale is None else scale, causal, window)
+    serving.attention_check()
     assert got.shape == q.shape and got.dtype == (dtype if out is None else out.dtype)
     err = (got.double() - want).abs()
     assert bool((err <= bound).all()), (float((err - bound).max()), float(err.max()))

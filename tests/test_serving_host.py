@@ -89,7 +89,7 @@ def test_empty_calls_do_nothing(lib):
     assert lib.dpuf_cuda_paged_attention(attn_args(n=0), None) == 0
     assert lib.dpuf_cuda_sample_rows(ADDR, 0, 8, 0, 8, ADDR, None, None, None, None, ADDR, None, None) == 0
     assert engine.last_error() == ""
-    for fn in (lib.dpuf_cuda_rope_append, lib.dpuf_cuda_paged_attention):
+    for fn in (lib.dpuf_cuda_rope_append, lib.dpuf_cuda_paged_attention, lib.dpuf_cuda_paged_attention_status):
         assert fn(None, None) == -1
 
 
