@@ -44,6 +44,7 @@ CUDA_SOURCES = [
     "kernels_rope.cu",
     "kernels_paged_attn.cu",
     "kernels_paged_attn_tc.cu",
+    "kernels_paged_attn_rows.cu",
     "kernels_sample.cu",
     "ops_serving.cu",
 ]

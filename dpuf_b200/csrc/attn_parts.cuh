@@ -38,6 +38,15 @@ DPUF_DEV int attn_arrive(unsigned* counter, int parts) {
   return last;
 }
 
+// True in the CTA that has to join the item's parts; all of its threads see the others' parts.
+DPUF_DEV bool attn_last_part(unsigned* counter, int parts, int* flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) *flag = attn_arrive(counter, parts);
+  __syncthreads();
+  return *flag != 0;
+}
+
 // Raises a kernel's dynamic shared-memory limit on its first launch on each device.
 template <auto kernel>
 cudaError_t smem_limit_once(int bytes) {
@@ -53,5 +62,7 @@ cudaError_t smem_limit_once(int bytes) {
 // 16-bit queries and cache, head_dim <= 128 (kernels_paged_attn_tc.cu).
 cudaError_t launch_paged_attention_tc(const AttnArgs& p, cudaStream_t s);
 size_t paged_attention_tc_workspace();
+// 16-bit cache, queries of its type or (head_dim <= 128) fp32 (kernels_paged_attn_rows.cu).
+cudaError_t launch_paged_attention_rows(const AttnArgs& p, cudaStream_t s);
 
 }  // namespace dpuf

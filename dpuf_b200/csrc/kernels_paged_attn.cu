@@ -24,15 +24,6 @@ DPUF_DEV float ex2(float x) {
   return y;
 }
 
-// True in the CTA that has to join the item's parts; all of its threads see the others' parts.
-DPUF_DEV bool attn_last_part(unsigned* counter, int parts, int* flag) {
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) *flag = attn_arrive(counter, parts);
-  __syncthreads();
-  return *flag != 0;
-}
-
 // ------------------------------------------------------------------ fp32 arithmetic, any types
 // A CTA takes 16 rows and blocks of 32 keys, both widened to fp32 in shared memory.  Thread
 // (row = tid / 16, x = tid % 16) has the scores of keys x and x + 16 and the output's dimensions
@@ -204,13 +195,6 @@ cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <typename TK>
-cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
-  if (p.a.kv.head_dim <= 64) return launch_f32<TK, 64>(p, s);
-  if (p.a.kv.head_dim <= 128) return launch_f32<TK, 128>(p, s);
-  return launch_f32<TK, 256>(p, s);
-}
-
 }  // namespace
 
 int64_t paged_attention_workspace() {
@@ -232,11 +216,15 @@ cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t
   p.group = a.n_q / a.kv.n_kv;
   p.page_shift = 31 - __builtin_clz((unsigned)a.kv.page_size);
   p.max_kv = (int)std::min<int64_t>((int64_t)a.pages_per_seq << p.page_shift, 1 << 30);
-  if (a.dtype == a.kv.dtype && a.dtype != DPUF_TYPE_F32 && a.kv.head_dim <= 128 && a.max_q * p.group > 16)
-    return launch_paged_attention_tc(p, s);
-  if (a.kv.dtype == DPUF_TYPE_F32) return launch_f32<float>(p, s);
-  if (a.kv.dtype == DPUF_TYPE_F16) return launch_f32<__half>(p, s);
-  return launch_f32<__nv_bfloat16>(p, s);
+  if (a.kv.dtype == DPUF_TYPE_F32) {
+    if (a.kv.head_dim <= 64) return launch_f32<float, 64>(p, s);
+    if (a.kv.head_dim <= 128) return launch_f32<float, 128>(p, s);
+    return launch_f32<float, 256>(p, s);
+  }
+  if (a.dtype == DPUF_TYPE_F32 && a.kv.head_dim > 128)
+    return a.kv.dtype == DPUF_TYPE_F16 ? launch_f32<__half, 256>(p, s) : launch_f32<__nv_bfloat16, 256>(p, s);
+  if (a.dtype != DPUF_TYPE_F32 && a.kv.head_dim <= 128 && a.max_q * p.group > 16) return launch_paged_attention_tc(p, s);
+  return launch_paged_attention_rows(p, s);
 }
 
 }  // namespace dpuf

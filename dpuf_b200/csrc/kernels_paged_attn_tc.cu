@@ -40,6 +40,9 @@ constexpr int kTile = 128;            // rows of a tile, keys of a block
 constexpr int kItemRows = 2 * kTile;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 320;
+// The weights carry a factor 2^7, and so does their sum: at most 2^15, which fp16 holds, while the
+// small ones of a long context keep their bits.
+constexpr float kLift = 7.0f;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 DPUF_DEV uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
             }
           }
         }
-        const float ref = m == -CUDART_INF_F ? 0.0f : m * sl;
+        const float ref = m == -CUDART_INF_F ? 0.0f : __fmaf_rn(m, sl, -kLift);
         float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kTile; i += 2) {
@@ -507,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       if (!whole) {
         const size_t slot = 2 * (size_t)blockIdx.x + (from == 0 ? 1 : 0);
         const int pr = w * kTile + t;
-        parts.ml[slot * kItemRows + pr] = make_float2(m * sl, l);
+        parts.ml[slot * kItemRows + pr] = make_float2(m == -CUDART_INF_F ? m : m * sl, l);
 #pragma unroll
         for (int i = 0; i < DP / 32; i++) {
           uint32_t o[32];

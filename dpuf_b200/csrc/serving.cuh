@@ -83,6 +83,19 @@ DPUF_DEV void store8_as(void* p, size_t i, int dtype, const float (&v)[8]) {
   *(uint4*)((uint16_t*)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Four consecutive elements, index i of p with i a multiple of 4 and p 16-byte aligned.
+DPUF_DEV void store4_as(void* p, size_t i, int dtype, float a, float b, float c, float d) {
+  if (dtype == DPUF_TYPE_F32) {
+    *(float4*)((float*)p + i) = make_float4(a, b, c, d);
+  } else if (dtype == DPUF_TYPE_F16) {
+    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+    *(uint2*)((__half*)p + i) = make_uint2(*(const uint32_t*)&x, *(const uint32_t*)&y);
+  } else {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+    *(uint2*)((__nv_bfloat16*)p + i) = make_uint2(*(const uint32_t*)&x, *(const uint32_t*)&y);
+  }
+}
+
 // ---- launchers (arguments checked by the callers in ops_serving.cu)
 cudaError_t launch_rope_append(const DpufRopeAppendArgs& a, bool vectors, cudaStream_t s);
 cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t s);
