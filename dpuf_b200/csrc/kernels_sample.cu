@@ -4,21 +4,27 @@
 // With m the row's maximum, an entry's weight is w = exp((l - m) / T) in fp32, taken into sums
 // as the integer f = round(w 2^43): sums of integers do not depend on their order, so neither do
 // the thresholds and the id (an entry below 2^-44 of the maximum's weight has f = 0 and is never
-// kept).  The entries kept by top-k and by top-p are the first ones in the order (logit down,
-// index up), i.e. all entries above a threshold value and the first few, by index, of those
-// equal to it.  The thresholds come from histograms of counts and weights instead of a sort: one
-// over 2,048 equal steps of (m - l) / T, then, inside the step that holds the threshold, over
-// ranges of the value's bits (made monotone) until the range is one value.
+// kept).  All three filters keep a prefix of the order (logit down, index up), i.e. all entries
+// above a threshold value and the first few, by index, of those equal to it.  No sort of the row:
 //
-// A row is read from memory once: the cluster's CTAs keep a slice each in shared memory, and
-// exchange histograms and running sums through distributed shared memory.  Each CTA adds up one
-// segment of the bins over all CTAs, then all look the threshold's bin up in the segments.
+//  1. the row's slices go to the cluster's shared memory, once; the maximum.
+//  2. a histogram of counts over 1,024 equal steps of (m - l) / T, summed over the cluster.  The
+//     step in which top-k ends follows exactly, for top-p a step by which it has ended for sure
+//     (a step's weight is between its count times its ends' weights), for min-p the same.
+//  3. the entries up to that step are compacted, in index order: mostly a few dozen.
+//  4. up to 512 of them: one CTA sorts them and applies the filters on running sums.  More: the
+//     threshold is searched by histograms of counts and weights over ranges of the value's bits
+//     (made monotone), each range the bin of the one before, until it is one value.
+//  5. the running weight in index order passes u times the kept weight at the id.
+//
+// Bound by latency for few rows (the cluster's barriers, about 0.6 us each), by the passes over
+// the slices for many; the row is read from memory once.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include <algorithm>
 
-#include "serving.cuh"
+#include "attn_parts.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -28,8 +34,10 @@ namespace {
 
 constexpr int kSampThreads = 512;
 constexpr int kSampWarps = kSampThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kMaxCluster = 8;
+constexpr int kBins = 1024;
+constexpr int kMaxCluster = 16;
+constexpr int kListCap = 1024;            // entries of a CTA's compacted list
+constexpr int kSortCap = kSampThreads;    // entries that one CTA sorts
 constexpr float kFix = 8796093022208.0f;  // 2^43
 constexpr float kReach = 30.6f;           // > 44 ln 2: beyond it f is 0
 
@@ -56,37 +64,54 @@ struct SampleArgs {
   float* probs;
 };
 
-struct Found {  // the bin in which a running sum passes its target, and the sums above it
-  int bin;
+struct Found {  // the bin in which a running sum reaches its target, and the sums above it
+  int bin;      // -1: not reached
   uint32_t count, above;
   u64 mass_above, mass;
 };
 
 struct SampleShared {
-  uint32_t count[kBins], m0[kBins], m1[kBins], m2[kBins];  // weights in three parts of 15 bits
-  uint32_t seg_count[kBins];                               // this CTA's segment, summed over the CTAs
+  uint32_t count[kBins];
+  union {
+    struct {
+      uint32_t m0[kBins], m1[kBins], m2[kBins];  // weights in three parts of 15 bits
+    };
+    u64 sorted[kSortCap];
+  };
+  uint32_t seg_count[kBins];  // this CTA's segment of the bins, summed over the CTAs
   u64 seg_mass[kBins];
+  float list_v[kListCap];
+  int list_i[kListCap];
   uint32_t seg_count_sum;
+  int list_n;
   u64 seg_mass_sum;
-  u64 best;           // maximum's key and lowest index
-  u64 exchange[2];
+  u64 best;  // maximum's key and lowest index
+  u64 exchange[4];
   u64 warp_sum[kSampWarps];
+  double warp_lo[kSampWarps], warp_hi[kSampWarps];
   Found found;
-  int pick;
-  float pick_w;
+  int step_k, step_p;
+  double hi_k;
 };
 
-DPUF_DEV u64 block_inclusive(u64 v, u64* warp_sum) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+DPUF_DEV u64 warp_inclusive(u64 v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const u64 t = __shfl_up_sync(kFull, v, o);
     if (lane >= o) v += t;
   }
+  return v;
+}
+DPUF_DEV u64 block_inclusive(u64 v, u64* warp_sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_inclusive(v);
   __syncthreads();
   if (lane == 31) warp_sum[warp] = v;
   __syncthreads();
-  for (int w = 0; w < warp; w++) v += warp_sum[w];
+#pragma unroll
+  for (int w = 0; w < kSampWarps; w++)
+    if (w < warp) v += warp_sum[w];
   return v;
 }
 DPUF_DEV u64 block_sum(u64 v, u64* warp_sum) {
@@ -96,6 +121,7 @@ DPUF_DEV u64 block_sum(u64 v, u64* warp_sum) {
   if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0;
+#pragma unroll
   for (int w = 0; w < kSampWarps; w++) v += warp_sum[w];
   return v;
 }
@@ -108,30 +134,71 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   cg::cluster_group cl = cg::this_cluster();
   const int R = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int row = blockIdx.x / R;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const T* src = (const T*)a.logits + (int64_t)row * a.row_stride;
   const int base = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - base);
   src += base;
   auto at = [&](int i) { return to_f32(i < a.cached ? cache[i] : src[i]); };
+  auto of = [&](int r) { return cl.map_shared_rank(&sh, r); };
+  // a sum over the cluster of a u64 that each CTA has in exchange[e] (after a cluster barrier)
+  auto over_cluster = [&](int e) {
+    u64 v = lane < R ? of(lane)->exchange[e] : 0;
+#pragma unroll
+    for (int o = kMaxCluster / 2; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return __shfl_sync(kFull, v, 0);
+  };
+  // and the sum of the lower ranks' only
+  auto below_rank = [&](int e) {
+    u64 v = lane < rank ? of(lane)->exchange[e] : 0;
+#pragma unroll
+    for (int o = kMaxCluster / 2; o; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return __shfl_sync(kFull, v, 0);
+  };
 
-  // ---- the slice, and the row's maximum (lowest index)
-  u64 best = 0;
-  for (int i = tid; i < n; i += kSampThreads) {
+  // ---- 1. the slice, and the row's maximum (lowest index)
+  float top_v = -CUDART_INF_F;
+  int top_i = -1;
+  auto see = [&](float v, int i) {
+    if (v > top_v) {
+      top_v = v;
+      top_i = i;
+    }
+  };
+  const bool vectors = ((uintptr_t)src & 15) == 0;
+  constexpr int kVec = 16 / sizeof(T);
+  const int in_vectors = vectors ? min(n, a.cached) / kVec * kVec : 0;
+#pragma unroll 4
+  for (int i = tid * kVec; i < in_vectors; i += kSampThreads * kVec) {
+    const uint4 x = __ldcs((const uint4*)(src + i));
+    *(uint4*)(cache + i) = x;
+    const T* e = (const T*)&x;
+#pragma unroll
+    for (int j = 0; j < kVec; j++) see(to_f32(e[j]), i + j);
+  }
+#pragma unroll 8
+  for (int i = in_vectors + tid; i < n; i += kSampThreads) {
     const T v = src[i];
     if (i < a.cached) cache[i] = v;
-    const u64 k = ((u64)value_key(to_f32(v)) << 32) | (uint32_t)~(uint32_t)(base + i);
-    best = max(best, k);
+    see(to_f32(v), i);
   }
+  // an empty thread's key is 0 (that of NaN); the lowest index wins among equal keys
+  u64 best = top_i < 0 ? 0 : ((u64)value_key(top_v) << 32) | (uint32_t)~(uint32_t)(base + top_i);
 #pragma unroll
   for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
-  if ((tid & 31) == 0) sh.warp_sum[tid >> 5] = best;
+  if (lane == 0) sh.warp_sum[tid >> 5] = best;
+  for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 0; w < kSampWarps; w++) best = max(best, sh.warp_sum[w]);
-    sh.best = best;
+  if (tid < 32) {
+    best = lane < kSampWarps ? sh.warp_sum[lane] : 0;
+#pragma unroll
+    for (int o = kSampWarps / 2; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
+    if (lane == 0) sh.best = best;
   }
   cl.sync();
-  for (int r = 0; r < R; r++) best = max(best, cl.map_shared_rank(&sh, r)->best);
+  best = lane < R ? of(lane)->best : 0;
+#pragma unroll
+  for (int o = kMaxCluster / 2; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
+  best = __shfl_sync(kFull, best, 0);
   const uint32_t key_max = (uint32_t)(best >> 32);
   const float m = key_value(key_max);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
@@ -148,24 +215,223 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   const int k = a.top_k ? a.top_k[row] : 0;
   const float top_p = a.top_p ? a.top_p[row] : 1.0f;
   const float min_p = fminf(a.min_p ? a.min_p[row] : 0.0f, 1.0f);
+  const float u = a.u[row];
   auto weight = [&](float v) {
     const float w = v == m ? 1.0f : expf((v - m) * inv_t);
     return w > 0.0f ? w : 0.0f;  // NaN has none
   };
   auto fixed = [&](float w) { return (u64)__float2ull_rn(w * kFix); };
-  const float step = (float)kBins / kReach * inv_t;  // bins per unit of m - l
-  auto first_bin = [&](float v) { return v == m ? 0 : (int)fminf((m - v) * step, (float)(kBins - 1)); };
+  const float per_step = (float)kBins / kReach;  // steps per unit of (m - l) / T
+  auto step_of = [&](float v) {                  // -1: beyond the reach, or NaN
+    const float z = v == m ? 0.0f : (m - v) * inv_t;
+    return z < kReach ? min((int)(z * per_step), kBins - 1) : -1;
+  };
+  auto finish = [&](int id, float w, u64 total) {
+    a.ids[row] = id;
+    if (a.probs) a.probs[row] = (float)((double)w * (double)kFix / (double)total);
+  };
 
-  // ---- histogram of the entries that `bin` gives a bin (>= 0), summed over the cluster
-  const int seg = kBins / R;
-  auto histogram = [&](auto bin) {
-    for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = sh.m0[b] = sh.m1[b] = sh.m2[b] = 0;
-    __syncthreads();
+  // ---- 2. the step by which the kept prefix has ended
+  const bool limit_k = k >= 1 && k < a.vocab, limit_p = top_p < 1.0f;
+  bool by_k = false, by_p = false;  // filters that may end the prefix
+  u64 mass = 0;                     // weight of what top-k keeps, where by_p
+  int last_step = kBins;            // kBins: the whole slice stays the domain
+  if (limit_k || limit_p) {
+    u64 mine = 0;
+    const bool want_mass = limit_p && !limit_k;
     for (int i = tid; i < n; i += kSampThreads) {
       const float v = at(i);
+      const int b = step_of(v);
+      if (b >= 0) {
+        atomicAdd(&sh.count[b], 1u);
+        if (want_mass) mine += fixed(weight(v));
+      }
+    }
+    if (want_mass) {
+      mine = block_sum(mine, sh.warp_sum);
+      if (tid == 0) sh.exchange[0] = mine;
+    }
+    cl.sync();
+    if (want_mass) mass = over_cluster(0);
+    // bins 2 tid and 2 tid + 1: counts, and bounds of their weights
+    uint32_t c[2] = {0, 0};
+#pragma unroll 8
+    for (int r = 0; r < R; r++) {
+      const uint2 x = *(const uint2*)&of(r)->count[2 * tid];
+      c[0] += x.x;
+      c[1] += x.y;
+    }
+    double lo[2], hi[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int b = 2 * tid + e;
+      hi[e] = c[e] * (double)(b == 0 ? 1.0f : expf(-(float)b / per_step) * 1.0001f);
+      lo[e] = b == kBins - 1 ? 0.0 : c[e] * (double)(expf(-(float)(b + 1) / per_step) * 0.9999f);
+    }
+    u64 cc = block_inclusive((u64)c[0] + c[1], sh.warp_sum);
+    double cl_ = lo[0] + lo[1], ch = hi[0] + hi[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(kFull, cl_, o), y = __shfl_up_sync(kFull, ch, o);
+      if (lane >= o) {
+        cl_ += x;
+        ch += y;
+      }
+    }
+    if (lane == 31) {
+      sh.warp_lo[tid >> 5] = cl_;
+      sh.warp_hi[tid >> 5] = ch;
+    }
+    if (tid == 0) sh.step_k = sh.step_p = kBins;
+    __syncthreads();
+    for (int w = 0; w < (tid >> 5); w++) {
+      cl_ += sh.warp_lo[w];
+      ch += sh.warp_hi[w];
+    }
+    // running sums at the ends of bins 2 tid and 2 tid + 1
+    const u64 run[2] = {cc - c[1], cc};
+    const double run_lo[2] = {cl_ - lo[1], cl_}, run_hi[2] = {ch - hi[1], ch};
+    if (limit_k)
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        if (run[e] > (u64)k && run[e] - c[e] <= (u64)k) {  // strictly more than k up to here
+          sh.step_k = 2 * tid + e;
+          sh.hi_k = run_hi[e];
+        }
+    __syncthreads();
+    by_k = limit_k && sh.step_k < kBins;
+    by_p = limit_p;
+    if (by_p && limit_k && !by_k) {  // the weight of everything is needed after all
+      u64 mine2 = 0;
+      for (int i = tid; i < n; i += kSampThreads) mine2 += fixed(weight(at(i)));
+      mine2 = block_sum(mine2, sh.warp_sum);
+      if (tid == 0) sh.exchange[0] = mine2;
+      cl.sync();
+      mass = over_cluster(0);
+    }
+    if (by_p) {
+      // at most the upper bound of top-k's weight where it is not known yet
+      const double target = (double)top_p * (by_k ? sh.hi_k : (double)mass / (double)kFix) * 1.0001;
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        if (run_lo[e] >= target && run_lo[e] - lo[e] < target) atomicMin(&sh.step_p, 2 * tid + e);
+      __syncthreads();
+    }
+    // top-p after a top-k that ends the prefix needs all that top-k keeps for its weight
+    last_step = by_k ? sh.step_k : sh.step_p;
+    if (min_p > 0.0f && !(by_k && by_p)) last_step = min(last_step, (int)(-logf(min_p) * per_step * 1.0001f) + 1);
+  }
+
+  // ---- 3. the entries up to that step, in index order (contiguous runs of odd length per thread:
+  // no bank conflicts)
+  const int per = ((n + kSampThreads - 1) / kSampThreads) | 1;
+  const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  bool listed = false;
+  if (last_step < kBins) {
+    uint32_t mine = 0;
+    for (int i = i0; i < i1; i++) mine += (unsigned)step_of(at(i)) <= (unsigned)last_step;
+    const uint32_t incl = (uint32_t)block_inclusive(mine, sh.warp_sum);
+    if (incl <= kListCap) {
+      uint32_t o = incl - mine;
+      if (mine)
+        for (int i = i0; i < i1; i++) {
+          const float v = at(i);
+          if ((unsigned)step_of(v) <= (unsigned)last_step) {
+            sh.list_v[o] = v;
+            sh.list_i[o++] = base + i;
+          }
+        }
+    }
+    if (tid == kSampThreads - 1) {
+      sh.list_n = (int)incl;
+      sh.exchange[1] = incl;
+    }
+    cl.sync();
+    const u64 entries = over_cluster(1);
+    listed = sh.list_n <= kListCap;
+    if (entries <= kSortCap) {
+      // ---- 4a. few: rank 0 has them all, in index order
+      if (rank == 0) {
+        const int nl = lane < R ? of(lane)->list_n : 0;
+        const int ends = (int)warp_inclusive((u64)nl), have = (int)entries;
+        int mine_from = -1, mine_at = 0;
+        for (int r = 0; r < R; r++) {
+          const int end = __shfl_sync(kFull, ends, r), nr = __shfl_sync(kFull, nl, r);
+          if (tid >= end - nr && tid < end) {
+            mine_from = r;
+            mine_at = tid - (end - nr);
+          }
+        }
+        float v = 0.0f;
+        int id = -1;
+        if (mine_from >= 0) {
+          v = of(mine_from)->list_v[mine_at];
+          id = of(mine_from)->list_i[mine_at];
+        }
+        u64 x = mine_from < 0 ? 0 : ((u64)value_key(v) << 32) | (uint32_t)~(uint32_t)tid;
+        int size = 32;
+        while (size < have) size <<= 1;
+        // bitonic sort, largest first, an element per thread
+        for (int len = 2; len <= size; len <<= 1)
+          for (int s = len >> 1; s; s >>= 1) {
+            u64 y;
+            if (s >= 32) {
+              __syncthreads();
+              sh.sorted[tid] = x;
+              __syncthreads();
+              y = sh.sorted[tid ^ s];
+            } else {
+              y = __shfl_xor_sync(kFull, x, s);
+            }
+            const bool first = (tid & s) == 0, down = (tid & len) == 0 || len == size;
+            x = first == down ? max(x, y) : min(x, y);
+          }
+        // thread t has the entry of rank t: prefixes by count, weight and weight's share
+        const bool real = tid < have;
+        const float w = real ? weight(key_value((uint32_t)(x >> 32))) : 0.0f;
+        const u64 f = fixed(w);
+        const bool in_k = real && (!by_k || tid < k);
+        const u64 incl_f = block_inclusive(in_k ? f : 0, sh.warp_sum);
+        if (by_k && by_p) {
+          if (tid == kSampThreads - 1) sh.exchange[2] = incl_f;
+          __syncthreads();
+          mass = sh.exchange[2];
+        }
+        const bool keep = in_k && (!by_p || tid == 0 || (double)(incl_f - f) < (double)top_p * (double)mass) && w >= min_p;
+        // back in index order
+        __syncthreads();
+        if (real) sh.sorted[(uint32_t)~(uint32_t)x] = keep ? f : 0;
+        __syncthreads();
+        const u64 g = real ? sh.sorted[tid] : 0;
+        const u64 cdf = block_inclusive(g, sh.warp_sum);
+        if (tid == kSampThreads - 1) sh.exchange[2] = cdf;
+        __syncthreads();
+        const u64 total = sh.exchange[2];
+        const double target = (double)u * (double)total;
+        auto passed = [&](u64 c) { return (double)c > target || c >= total; };
+        if (g && passed(cdf) && !(cdf > g && passed(cdf - g))) finish(id, weight(v), total);
+      }
+      cl.sync();
+      return;
+    }
+  }
+
+  if (last_step == kBins) cl.sync();  // the counts are read: the histograms below may overwrite them
+
+  // ---- 4b. many: thresholds by histograms over the list, or the slice where the list is too long
+  const int dn = listed ? sh.list_n : n;
+  auto value = [&](int i) { return listed ? sh.list_v[i] : at(i); };
+  const int seg = kBins / R;
+  auto histogram = [&](uint32_t lo, uint32_t hi, int shift) {
+    for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = sh.m0[b] = sh.m1[b] = sh.m2[b] = 0;
+    __syncthreads();
+    for (int i = tid; i < dn; i += kSampThreads) {
+      const float v = value(i);
+      const uint32_t kv = value_key(v);
+      if (kv < lo || kv > hi) continue;
       const u64 f = fixed(weight(v));
-      const int b = f ? bin(v) : -1;
-      if (b < 0) continue;
+      if (!f) continue;
+      const int b = (int)((hi - kv) >> shift);
       atomicAdd(&sh.count[b], 1u);
       atomicAdd(&sh.m0[b], (uint32_t)f & 0x7FFF);
       atomicAdd(&sh.m1[b], (uint32_t)(f >> 15) & 0x7FFF);
@@ -176,8 +442,9 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     for (int b = tid; b < seg; b += kSampThreads) {
       uint32_t c = 0;
       u64 f = 0;
+#pragma unroll 4
       for (int r = 0; r < R; r++) {
-        const SampleShared* o = cl.map_shared_rank(&sh, r);
+        const SampleShared* o = of(r);
         const int g = rank * seg + b;
         c += o->count[g];
         f += (u64)o->m0[g] + ((u64)o->m1[g] << 15) + ((u64)o->m2[g] << 30);
@@ -195,155 +462,119 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     }
     cl.sync();
   };
-  // ---- the bin in which the count (by_count) or the weight reaches the target
-  auto find = [&](bool by_count, uint32_t count0, u64 mass0, uint32_t k_target, double p_target) {
+  // the bin in which the count (by_count) or the weight reaches the target, from the sums above
+  auto find = [&](bool by_count, const Found& above, uint32_t k_target, double p_target) {
     __syncthreads();
     if (tid < 32) {
-      uint32_t c = count0;
-      u64 f = mass0;
-      auto reached = [&](uint32_t cc, u64 ff) { return by_count ? cc >= k_target : (double)ff >= p_target; };
-      int r = 0;
-      for (; r < R - 1; r++) {
-        const SampleShared* o = cl.map_shared_rank(&sh, r);
-        if (reached(c + o->seg_count_sum, f + o->seg_mass_sum)) break;
-        c += o->seg_count_sum;
-        f += o->seg_mass_sum;
-      }
-      // a lane's run of bins, then the bin within the run
-      const SampleShared* o = cl.map_shared_rank(&sh, r);
-      const int per = seg / 32;
-      uint32_t lc = 0;
-      u64 lf = 0;
-      for (int b = 0; b < per; b++) {
-        lc += o->seg_count[tid * per + b];
-        lf += o->seg_mass[tid * per + b];
-      }
-      uint32_t ic = lc;
-      u64 jf = lf;
-#pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const uint32_t tc = __shfl_up_sync(kFull, ic, s);
-        const u64 tf = __shfl_up_sync(kFull, jf, s);
-        if (tid >= s) {
-          ic += tc;
-          jf += tf;
-        }
-      }
-      const unsigned hit = __ballot_sync(kFull, reached(c + ic, f + jf) && lc > 0);
-      const unsigned any = __ballot_sync(kFull, lc > 0);
-      const int lane = hit ? __ffs(hit) - 1 : any ? 31 - __clz(any) : 0;
-      if (tid == lane) {
-        c += ic - lc;
-        f += jf - lf;
-        int b = 0, last = 0;
-        uint32_t c2 = c, lastc = c;
-        u64 f2 = f, lastf = f;
-        for (; b < per; b++) {
-          const uint32_t bc = o->seg_count[tid * per + b];
-          const u64 bf = o->seg_mass[tid * per + b];
-          if (bc) {
-            last = b;
-            lastc = c2;
-            lastf = f2;
-            if (reached(c2 + bc, f2 + bf)) break;
+      auto reached = [&](u64 cc, u64 ff) { return by_count ? cc >= k_target : (double)ff >= p_target; };
+      const u64 c0 = lane < R ? of(lane)->seg_count_sum : 0, f0 = lane < R ? of(lane)->seg_mass_sum : 0;
+      const u64 ci = warp_inclusive(c0) + above.above, fi = warp_inclusive(f0) + above.mass_above;
+      const unsigned in = __ballot_sync(kFull, lane < R && c0 > 0 && reached(ci, fi));
+      Found f{-1, 0, 0, 0, 0};
+      if (in) {
+        const int r = __ffs(in) - 1;
+        u64 c = __shfl_sync(kFull, ci - c0, r), g = __shfl_sync(kFull, fi - f0, r);
+        const SampleShared* o = of(r);
+        for (int b = 0; b < seg; b += 32) {  // 32 bins at a time
+          const u64 bc = b + lane < seg ? o->seg_count[b + lane] : 0, bf = b + lane < seg ? o->seg_mass[b + lane] : 0;
+          const u64 ic = warp_inclusive(bc) + c, jf = warp_inclusive(bf) + g;
+          const unsigned hit = __ballot_sync(kFull, bc > 0 && reached(ic, jf));
+          if (hit) {
+            const int x = __ffs(hit) - 1;
+            f.bin = r * seg + b + x;
+            f.count = (uint32_t)__shfl_sync(kFull, bc, x);
+            f.mass = __shfl_sync(kFull, bf, x);
+            f.above = (uint32_t)__shfl_sync(kFull, ic - bc, x);
+            f.mass_above = __shfl_sync(kFull, jf - bf, x);
+            break;
           }
-          c2 += bc;
-          f2 += bf;
+          c = __shfl_sync(kFull, ic, 31);
+          g = __shfl_sync(kFull, jf, 31);
         }
-        sh.found = Found{r * seg + tid * per + last, o->seg_count[tid * per + last], lastc, lastf,
-                         o->seg_mass[tid * per + last]};
       }
+      if (tid == 0) sh.found = f;
     }
     __syncthreads();
     return sh.found;
   };
-  // ---- from the first histogram's bin to one value: its key, and what lies above it
-  auto refine = [&](Found f1, bool by_count, uint32_t k_target, double p_target, uint32_t* key, Found* cls) {
-    const int b1 = f1.bin;
-    const float lo_v = m - (float)(b1 + 1) / step, hi_v = m - (float)b1 / step;
-    const float slack = 1e-5f * (fabsf(m) + fabsf(lo_v)) + 1e-30f;
-    uint32_t hi = b1 == 0 ? key_max : min(key_max, value_key(hi_v + slack));
-    uint32_t lo = b1 == kBins - 1 ? 1u : value_key(lo_v - slack);
-    if (!(lo_v - slack <= hi_v + slack)) lo = 1u, hi = key_max;  // m or the step is not finite
-    Found f = f1;
+  // the value in which the target is reached: its key, the sums above it and its own (bin -1: not
+  // reached in the domain)
+  auto select = [&](bool by_count, uint32_t k_target, double p_target, uint32_t* key) {
+    uint32_t hi = key_max, lo = 1;
+    if (last_step < kBins) {  // nothing of the domain is below this step's end
+      const float low = m - (float)(last_step + 1) / per_step * temp;
+      const float slack = 1e-5f * (fabsf(m) + fabsf(low)) + 1e-30f;
+      if (low - slack <= m) lo = max(1u, value_key(low - slack));
+    }
+    Found f{0, 0, 0, 0, 0};
     for (;;) {
       int shift = 0;
       while (((hi - lo) >> shift) >= (uint32_t)kBins) shift++;
-      histogram([&](float v) {
-        const uint32_t kv = value_key(v);
-        return first_bin(v) == b1 && kv >= lo && kv <= hi ? (int)((hi - kv) >> shift) : -1;
-      });
-      f = find(by_count, f.above, f.mass_above, k_target, p_target);
+      histogram(lo, hi, shift);
+      f = find(by_count, f, k_target, p_target);
+      if (f.bin < 0) return f;
       const uint32_t top = hi - ((uint32_t)f.bin << shift);
       if (shift == 0) {
         *key = top;
-        *cls = f;
-        return;
+        return f;
       }
-      lo = max(lo, top - ((1u << shift) - 1));
+      const uint32_t width = (1u << shift) - 1;
+      lo = top - lo > width ? top - width : lo;
       hi = top;
     }
   };
-
   uint32_t key_t = 0;          // kept: keys above it,
   uint32_t ties = 0xFFFFFFFFu;  // and the first `ties` entries equal to it
-  const bool limit_k = k >= 1 && k < a.vocab, limit_p = top_p < 1.0f;
-  if (limit_k || limit_p) {
-    histogram(first_bin);
-    uint32_t count = 0;
-    u64 mass = 0;
-    for (int r = 0; r < R; r++) {
-      const SampleShared* o = cl.map_shared_rank(&sh, r);
-      count += o->seg_count_sum;
-      mass += o->seg_mass_sum;
+  if (by_k) {
+    const Found f = select(true, (uint32_t)k, 0.0, &key_t);
+    if (f.bin >= 0) {
+      ties = (uint32_t)k - f.above;
+      mass = f.mass_above + f.mass / f.count * ties;
+    } else {  // fewer than k have any weight: the list holds all of them
+      by_k = false;
+      u64 mine = 0;
+      for (int i = tid; i < dn; i += kSampThreads) mine += fixed(weight(value(i)));
+      mine = block_sum(mine, sh.warp_sum);
+      if (tid == 0) sh.exchange[0] = mine;
+      cl.sync();
+      mass = over_cluster(0);
     }
-    const bool by_k = limit_k && (uint32_t)k < count;
-    Found fk{}, fp{};
-    if (by_k) fk = find(true, 0, 0, (uint32_t)k, 0.0);
-    // the weight that top-p has to hold is known once top-k's threshold is: both start from the
-    // first histogram, so the refinements (which overwrite it) come after the look-ups
-    if (!by_k) {
-      if (limit_p && top_p > 0.0f) fp = find(false, 0, 0, 0, (double)top_p * (double)mass);
+  }
+  if (by_p) {
+    const double target = (double)top_p * (double)mass;
+    if (!(target > 0.0)) {
+      key_t = key_max;
+      ties = 1;
     } else {
-      Found cls;
-      refine(fk, true, (uint32_t)k, 0.0, &key_t, &cls);
-      ties = (uint32_t)k - cls.above;
-      mass = cls.mass_above + cls.mass / cls.count * ties;
-      if (limit_p && top_p > 0.0f) {
-        histogram(first_bin);
-        fp = find(false, 0, 0, 0, (double)top_p * (double)mass);
-      }
-    }
-    if (limit_p) {
-      if (!(top_p > 0.0f)) {
-        key_t = key_max;
-        ties = 1;
-      } else {
-        const double target = (double)top_p * (double)mass;
-        Found cls;
-        refine(fp, false, 0, target, &key_t, &cls);
-        const u64 each = cls.mass / cls.count;
+      uint32_t key_p = 0;
+      const Found f = select(false, 0, target, &key_p);
+      if (f.bin >= 0) {
+        const u64 each = f.mass / f.count;
         // the fewest of the class that reach the target
-        u64 c = (double)cls.mass_above >= target ? 1 : (u64)((target - (double)cls.mass_above) / (double)each);
-        while (c > 1 && (double)(cls.mass_above + (c - 1) * each) >= target) c--;
-        while (c < cls.count && (double)(cls.mass_above + c * each) < target) c++;
-        ties = (uint32_t)max((u64)1, c);
+        u64 c = (double)f.mass_above >= target ? 1 : (u64)((target - (double)f.mass_above) / (double)each);
+        while (c > 1 && (double)(f.mass_above + (c - 1) * each) >= target) c--;
+        while (c < f.count && (double)(f.mass_above + c * each) < target) c++;
+        const uint32_t ties_p = (uint32_t)max((u64)1, c);
+        // the shorter of the two prefixes
+        if (key_p > key_t || (key_p == key_t && ties_p < ties)) {
+          key_t = key_p;
+          ties = ties_p;
+        }
       }
     }
   }
 
-  // ---- index order: a thread's run of the slice is contiguous, of odd length (no bank conflicts)
-  const int per = ((n + kSampThreads - 1) / kSampThreads) | 1;
-  const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  // ---- 5. index order: a thread's run of the domain is contiguous
+  const int dper = ((dn + kSampThreads - 1) / kSampThreads) | 1;
+  const int d0 = min(tid * dper, dn), d1 = min(d0 + dper, dn);
   uint32_t before = 0;  // entries equal to the threshold at lower indices
   if (ties != 0xFFFFFFFFu) {
     uint32_t mine = 0;
-    for (int i = i0; i < i1; i++) mine += value_key(at(i)) == key_t;
+    for (int i = d0; i < d1; i++) mine += value_key(value(i)) == key_t;
     const u64 incl = block_inclusive(mine, sh.warp_sum);
-    if (tid == kSampThreads - 1) sh.exchange[0] = incl;
+    if (tid == kSampThreads - 1) sh.exchange[3] = incl;
     cl.sync();
-    before = (uint32_t)incl - mine;
-    for (int r = 0; r < rank; r++) before += (uint32_t)cl.map_shared_rank(&sh, r)->exchange[0];
+    before = (uint32_t)(incl - mine + below_rank(3));
   }
   auto kept = [&](float v, uint32_t& tie) -> u64 {
     const uint32_t kv = value_key(v);
@@ -355,30 +586,24 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   u64 mine = 0;
   {
     uint32_t tie = before;
-    for (int i = i0; i < i1; i++) mine += kept(at(i), tie);
+    for (int i = d0; i < d1; i++) mine += kept(value(i), tie);
   }
   u64 incl = block_inclusive(mine, sh.warp_sum);
-  if (tid == kSampThreads - 1) sh.exchange[1] = incl;
+  if (tid == kSampThreads - 1) sh.exchange[2] = incl;
   cl.sync();
-  u64 total = 0, lower = 0;
-  for (int r = 0; r < R; r++) {
-    const u64 e = cl.map_shared_rank(&sh, r)->exchange[1];
-    if (r < rank) lower += e;
-    total += e;
-  }
-  incl += lower;
-  const double target = (double)a.u[row] * (double)total;
+  const u64 total = over_cluster(2);
+  incl += below_rank(2);
+  const double target = (double)u * (double)total;
   auto passed = [&](u64 c) { return (double)c > target || c >= total; };
   if (mine && passed(incl) && !(incl - mine > 0 && passed(incl - mine))) {  // one thread of the cluster
     u64 run = incl - mine;
     uint32_t tie = before;
-    for (int i = i0; i < i1; i++) {
-      const float v = at(i);
+    for (int i = d0; i < d1; i++) {
+      const float v = value(i);
       const u64 f = kept(v, tie);
       run += f;
       if (f && passed(run)) {
-        a.ids[row] = base + i;
-        if (a.probs) a.probs[row] = (float)((double)weight(v) * (double)kFix / (double)total);
+        finish(listed ? sh.list_i[i] : base + i, weight(v), total);
         break;
       }
     }
@@ -389,14 +614,25 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
 template <typename T>
 cudaError_t launch(const SampleArgs& args, cudaStream_t s) {
   SampleArgs a = args;
+  // CTAs per row: as many as keep about 2,048 entries each, while the grid leaves SMs idle up to
+  // 16 a row; then 8 of which two fit an SM.
   int cluster = 1;
-  while (cluster < kMaxCluster && a.vocab > cluster * 4096) cluster *= 2;
-  a.slice = (a.vocab + cluster - 1) / cluster;
+  while (cluster < kMaxCluster && a.vocab > cluster * 4096 && (cluster < 8 || a.rows * cluster * 2 <= 2 * kAttnSms))
+    cluster *= 2;
+  const int align = 16 / (int)sizeof(T);
+  a.slice = ((a.vocab + cluster - 1) / cluster + align - 1) / align * align;
   const size_t head = (sizeof(SampleShared) + 15) & ~(size_t)15;
   const size_t room = 200 * 1024 - head;
-  a.cached = (int)std::min((size_t)a.slice, room / sizeof(T));
+  a.cached = (int)std::min((size_t)a.slice, room / sizeof(T) / align * align);
   const size_t smem = head + (size_t)a.cached * sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static bool wide[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64 || !wide[dev])) {
+    e = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) wide[dev] = true;
+  }
+  if (e == cudaSuccess) e = smem_limit_once<sample_rows_kernel<T>>(200 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * cluster);
