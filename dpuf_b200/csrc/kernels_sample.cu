@@ -11,14 +11,17 @@
 //  2. a histogram of counts over 1,024 equal steps of (m - l) / T, summed over the cluster.  The
 //     step in which top-k ends follows exactly, for top-p a step by which it has ended for sure
 //     (a step's weight is between its count times its ends' weights), for min-p the same.
-//  3. the entries up to that step are compacted, in index order: mostly a few dozen.
-//  4. up to 512 of them: one CTA sorts them and applies the filters on running sums.  More: the
-//     threshold is searched by histograms of counts and weights over ranges of the value's bits
-//     (made monotone), each range the bin of the one before, until it is one value.
+//  3. the entries down to that step are compacted, in index order, and moved to one CTA of the
+//     cluster (the others are then done): mostly a few dozen.
+//  4. up to 512 of them it sorts, and applies the filters on running sums.  Of more, the thresholds
+//     are searched by histograms of counts and weights over ranges of the value's bits (made
+//     monotone), each range the bin of the one before, until it is one value.  Where they are too
+//     many to move (a nucleus of much of the vocabulary) the cluster does the same together, each
+//     CTA adding up one segment of the bins.
 //  5. the running weight in index order passes u times the kept weight at the id.
 //
-// Bound by latency for few rows (the cluster's barriers, about 0.6 us each), by the passes over
-// the slices for many; the row is read from memory once.
+// Bound by latency for few rows (the cluster's barriers and the block's), by the passes over the
+// slices for many; the row is read from memory once.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -36,25 +39,34 @@ constexpr int kSampThreads = 512;
 constexpr int kSampWarps = kSampThreads / 32;
 constexpr int kBins = 1024;
 constexpr int kMaxCluster = 16;
-constexpr int kListCap = 1024;            // entries of a CTA's compacted list
+constexpr int kListCap = 1024;            // entries that one CTA hands over
 constexpr int kSortCap = kSampThreads;    // entries that one CTA sorts
 constexpr float kFix = 8796093022208.0f;  // 2^43
 constexpr float kReach = 30.6f;           // > 44 ln 2: beyond it f is 0
 
 typedef unsigned long long u64;
 
-// Unsigned integers in the order of the values; NaN below everything.
-DPUF_DEV uint32_t value_key(float v) {
-  if (v != v) return 0;
-  const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);  // -0 equals 0
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
-DPUF_DEV float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
+// Unsigned integers in the order of the values (0 for NaN); of the 16-bit types without the low
+// bits that their fp32 form does not use, so that neighbouring values have neighbouring keys.
+template <typename T>
+struct Key {
+  static constexpr int drop = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+  static DPUF_DEV uint32_t of(float v) {
+    if (v != v) return 0;
+    const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);  // -0 equals 0
+    return ((b & 0x80000000u) ? ~b : b | 0x80000000u) >> drop;
+  }
+  static DPUF_DEV float value(uint32_t k) {
+    const uint32_t b = k << drop;
+    return __uint_as_float((b & 0x80000000u) ? b & 0x7FFFFFFFu : ~(b | ((1u << drop) - 1)));
+  }
+};
 
 struct SampleArgs {
   const void* logits;
   int64_t row_stride;
   int rows, vocab, slice, cached;  // cached: entries of a slice kept in shared memory
+  int given, given_i;              // entries that rank 0 can be given (in its slice's place), offset of their indices
   const float* u;
   const float* temperature;
   const int* top_k;
@@ -78,13 +90,12 @@ struct SampleShared {
     };
     u64 sorted[kSortCap];
   };
-  uint32_t seg_count[kBins];  // this CTA's segment of the bins, summed over the CTAs
-  u64 seg_mass[kBins];
+  uint32_t bin_count[kBins];  // this CTA's segment of the bins, summed over the CTAs
+  u64 bin_mass[kBins];
   float list_v[kListCap];
   int list_i[kListCap];
-  uint32_t seg_count_sum;
-  int list_n;
-  u64 seg_mass_sum;
+  uint32_t seg_count;
+  u64 seg_mass;
   u64 best;  // maximum's key and lowest index
   u64 exchange[4];
   u64 warp_sum[kSampWarps];
@@ -182,7 +193,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     see(to_f32(v), i);
   }
   // an empty thread's key is 0 (that of NaN); the lowest index wins among equal keys
-  u64 best = top_i < 0 ? 0 : ((u64)value_key(top_v) << 32) | (uint32_t)~(uint32_t)(base + top_i);
+  u64 best = top_i < 0 ? 0 : ((u64)Key<T>::of(top_v) << 32) | (uint32_t)~(uint32_t)(base + top_i);
 #pragma unroll
   for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
   if (lane == 0) sh.warp_sum[tid >> 5] = best;
@@ -200,10 +211,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   for (int o = kMaxCluster / 2; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
   best = __shfl_sync(kFull, best, 0);
   const uint32_t key_max = (uint32_t)(best >> 32);
-  const float m = key_value(key_max);
+  const float m = Key<T>::value(key_max);
   const float temp = a.temperature ? a.temperature[row] : 1.0f;
-  const bool nothing = key_max <= value_key(-CUDART_INF_F);
-  if (nothing || !(temp > 0.0f)) {
+  const bool nothing = key_max <= Key<T>::of(-CUDART_INF_F);
+  const int k = a.top_k ? a.top_k[row] : 0;
+  const float top_p = a.top_p ? a.top_p[row] : 1.0f;
+  if (nothing || !(temp > 0.0f) || k == 1 || top_p <= 0.0f) {  // the first maximum is all that is kept
     if (rank == 0 && tid == 0) {
       a.ids[row] = nothing ? -1 : (int)~(uint32_t)best;
       if (a.probs) a.probs[row] = nothing ? 0.0f : 1.0f;
@@ -212,8 +225,6 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     return;
   }
   const float inv_t = 1.0f / temp;
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const float top_p = a.top_p ? a.top_p[row] : 1.0f;
   const float min_p = fminf(a.min_p ? a.min_p[row] : 0.0f, 1.0f);
   const float u = a.u[row];
   auto weight = [&](float v) {
@@ -225,6 +236,17 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   auto step_of = [&](float v) {                  // -1: beyond the reach, or NaN
     const float z = v == m ? 0.0f : (m - v) * inv_t;
     return z < kReach ? min((int)(z * per_step), kBins - 1) : -1;
+  };
+  // every entry of the slice, in no order: 16 bytes at a time
+  auto each = [&](auto f) {
+    const int full = min(n, a.cached) / kVec * kVec;
+    for (int i = tid * kVec; i < full; i += kSampThreads * kVec) {
+      const uint4 x = *(const uint4*)(cache + i);
+      const T* e = (const T*)&x;
+#pragma unroll
+      for (int j = 0; j < kVec; j++) f(to_f32(e[j]));
+    }
+    for (int i = full + tid; i < n; i += kSampThreads) f(at(i));
   };
   auto finish = [&](int id, float w, u64 total) {
     a.ids[row] = id;
@@ -239,14 +261,13 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   if (limit_k || limit_p) {
     u64 mine = 0;
     const bool want_mass = limit_p && !limit_k;
-    for (int i = tid; i < n; i += kSampThreads) {
-      const float v = at(i);
+    each([&](float v) {
       const int b = step_of(v);
       if (b >= 0) {
         atomicAdd(&sh.count[b], 1u);
         if (want_mass) mine += fixed(weight(v));
       }
-    }
+    });
     if (want_mass) {
       mine = block_sum(mine, sh.warp_sum);
       if (tid == 0) sh.exchange[0] = mine;
@@ -303,7 +324,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     by_p = limit_p;
     if (by_p && limit_k && !by_k) {  // the weight of everything is needed after all
       u64 mine2 = 0;
-      for (int i = tid; i < n; i += kSampThreads) mine2 += fixed(weight(at(i)));
+      each([&](float v) { mine2 += fixed(weight(v)); });
       mine2 = block_sum(mine2, sh.warp_sum);
       if (tid == 0) sh.exchange[0] = mine2;
       cl.sync();
@@ -322,112 +343,118 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     if (min_p > 0.0f && !(by_k && by_p)) last_step = min(last_step, (int)(-logf(min_p) * per_step * 1.0001f) + 1);
   }
 
-  // ---- 3. the entries up to that step, in index order (contiguous runs of odd length per thread:
-  // no bank conflicts)
+  // ---- 3. the entries down to that step, in index order (a thread's run of the slice is
+  // contiguous and of odd length: no bank conflicts), moved to rank 0
   const int per = ((n + kSampThreads - 1) / kSampThreads) | 1;
   const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
-  bool listed = false;
+  float cut = -CUDART_INF_F;
+  bool local = false;  // rank 0 goes on alone, over what it has been given
+  int have = 0;
+  T* const given_v = cache;
+  int* const given_i = (int*)(dyn + a.given_i);
   if (last_step < kBins) {
+    const float low = m - (float)(last_step + 1) / per_step * temp;
+    cut = fminf(low - 1e-5f * (fabsf(m) + fabsf(low)) - 1e-30f, m);  // at or below every entry wanted
+    if (!(cut <= m)) cut = -CUDART_INF_F;                             // the step's end is not finite
     uint32_t mine = 0;
-    for (int i = i0; i < i1; i++) mine += (unsigned)step_of(at(i)) <= (unsigned)last_step;
+    for (int i = i0; i < i1; i++) mine += at(i) >= cut;
     const uint32_t incl = (uint32_t)block_inclusive(mine, sh.warp_sum);
-    if (incl <= kListCap) {
+    if (incl <= kListCap && mine) {
       uint32_t o = incl - mine;
-      if (mine)
-        for (int i = i0; i < i1; i++) {
-          const float v = at(i);
-          if ((unsigned)step_of(v) <= (unsigned)last_step) {
-            sh.list_v[o] = v;
-            sh.list_i[o++] = base + i;
-          }
+      for (int i = i0; i < i1; i++) {
+        const float v = at(i);
+        if (v >= cut) {
+          sh.list_v[o] = v;
+          sh.list_i[o++] = base + i;
         }
+      }
     }
-    if (tid == kSampThreads - 1) {
-      sh.list_n = (int)incl;
-      sh.exchange[1] = incl;
-    }
-    cl.sync();
+    if (tid == kSampThreads - 1) sh.exchange[1] = incl <= kListCap ? incl : 1u << 30;
+    cl.sync();  // rank 0's slice is not needed any more if the lists fit
     const u64 entries = over_cluster(1);
-    listed = sh.list_n <= kListCap;
-    if (entries <= kSortCap) {
-      // ---- 4a. few: rank 0 has them all, in index order
-      if (rank == 0) {
-        const int nl = lane < R ? of(lane)->list_n : 0;
-        const int ends = (int)warp_inclusive((u64)nl), have = (int)entries;
-        int mine_from = -1, mine_at = 0;
-        for (int r = 0; r < R; r++) {
-          const int end = __shfl_sync(kFull, ends, r), nr = __shfl_sync(kFull, nl, r);
-          if (tid >= end - nr && tid < end) {
-            mine_from = r;
-            mine_at = tid - (end - nr);
-          }
-        }
-        float v = 0.0f;
-        int id = -1;
-        if (mine_from >= 0) {
-          v = of(mine_from)->list_v[mine_at];
-          id = of(mine_from)->list_i[mine_at];
-        }
-        u64 x = mine_from < 0 ? 0 : ((u64)value_key(v) << 32) | (uint32_t)~(uint32_t)tid;
-        int size = 32;
-        while (size < have) size <<= 1;
-        // bitonic sort, largest first, an element per thread
-        for (int len = 2; len <= size; len <<= 1)
-          for (int s = len >> 1; s; s >>= 1) {
-            u64 y;
-            if (s >= 32) {
-              __syncthreads();
-              sh.sorted[tid] = x;
-              __syncthreads();
-              y = sh.sorted[tid ^ s];
-            } else {
-              y = __shfl_xor_sync(kFull, x, s);
-            }
-            const bool first = (tid & s) == 0, down = (tid & len) == 0 || len == size;
-            x = first == down ? max(x, y) : min(x, y);
-          }
-        // thread t has the entry of rank t: prefixes by count, weight and weight's share
-        const bool real = tid < have;
-        const float w = real ? weight(key_value((uint32_t)(x >> 32))) : 0.0f;
-        const u64 f = fixed(w);
-        const bool in_k = real && (!by_k || tid < k);
-        const u64 incl_f = block_inclusive(in_k ? f : 0, sh.warp_sum);
-        if (by_k && by_p) {
-          if (tid == kSampThreads - 1) sh.exchange[2] = incl_f;
-          __syncthreads();
-          mass = sh.exchange[2];
-        }
-        const bool keep = in_k && (!by_p || tid == 0 || (double)(incl_f - f) < (double)top_p * (double)mass) && w >= min_p;
-        // back in index order
-        __syncthreads();
-        if (real) sh.sorted[(uint32_t)~(uint32_t)x] = keep ? f : 0;
-        __syncthreads();
-        const u64 g = real ? sh.sorted[tid] : 0;
-        const u64 cdf = block_inclusive(g, sh.warp_sum);
-        if (tid == kSampThreads - 1) sh.exchange[2] = cdf;
-        __syncthreads();
-        const u64 total = sh.exchange[2];
-        const double target = (double)u * (double)total;
-        auto passed = [&](u64 c) { return (double)c > target || c >= total; };
-        if (g && passed(cdf) && !(cdf > g && passed(cdf - g))) finish(id, weight(v), total);
+    if (entries <= (u64)a.given) {
+      local = true;
+      have = (int)entries;
+      SampleShared* const to = of(0);
+      T* const tv = (T*)((unsigned char*)to + ((unsigned char*)given_v - dyn));
+      int* const ti = (int*)((unsigned char*)to + ((unsigned char*)given_i - dyn));
+      const int first = (int)below_rank(1), mine_n = (int)sh.exchange[1];
+      for (int i = tid; i < mine_n; i += kSampThreads) {
+        tv[first + i] = from_f32<T>(sh.list_v[i]);
+        ti[first + i] = sh.list_i[i];
       }
       cl.sync();
-      return;
+      if (rank != 0) return;
     }
+  } else if (limit_p) {
+    cl.sync();  // the counts are read: the histograms below may overwrite them
   }
 
-  if (last_step == kBins) cl.sync();  // the counts are read: the histograms below may overwrite them
+  if (local && have <= kSortCap) {
+    // ---- 4. few: sorted, largest first, an entry per thread (bitonic)
+    const bool real = tid < have;
+    const float v = real ? to_f32(given_v[tid]) : 0.0f;
+    const int id = real ? given_i[tid] : -1;
+    u64 x = real ? ((u64)Key<T>::of(v) << 32) | (uint32_t)~(uint32_t)tid : 0;
+    int size = 32;
+    while (size < have) size <<= 1;
+    for (int len = 2; len <= size; len <<= 1)
+      for (int s = len >> 1; s; s >>= 1) {
+        u64 y;
+        if (s >= 32) {
+          __syncthreads();
+          sh.sorted[tid] = x;
+          __syncthreads();
+          y = sh.sorted[tid ^ s];
+        } else {
+          y = __shfl_xor_sync(kFull, x, s);
+        }
+        const bool first = (tid & s) == 0, down = (tid & len) == 0 || len == size;
+        x = first == down ? max(x, y) : min(x, y);
+      }
+    // thread t has the entry of rank t: prefixes by count, by weight, by the weight's share
+    const float w = real ? weight(Key<T>::value((uint32_t)(x >> 32))) : 0.0f;
+    const u64 f = fixed(w);
+    const bool in_k = real && (!by_k || tid < k);
+    const u64 incl = block_inclusive(in_k ? f : 0, sh.warp_sum);
+    if (by_k && by_p) {
+      if (tid == kSampThreads - 1) sh.exchange[2] = incl;
+      __syncthreads();
+      mass = sh.exchange[2];
+    }
+    const bool keep = in_k && (!by_p || tid == 0 || (double)(incl - f) < (double)top_p * (double)mass) && w >= min_p;
+    // back in index order
+    __syncthreads();
+    if (real) sh.sorted[(uint32_t)~(uint32_t)x] = keep ? f : 0;
+    __syncthreads();
+    const u64 g = real ? sh.sorted[tid] : 0;
+    const u64 cdf = block_inclusive(g, sh.warp_sum);
+    if (tid == kSampThreads - 1) sh.exchange[3] = cdf;
+    __syncthreads();
+    const u64 total = sh.exchange[3];
+    const double target = (double)u * (double)total;
+    auto passed = [&](u64 c) { return (double)c > target || c >= total; };
+    if (g && passed(cdf) && !(cdf > g && passed(cdf - g))) finish(id, weight(v), total);
+    return;
+  }
 
-  // ---- 4b. many: thresholds by histograms over the list, or the slice where the list is too long
-  const int dn = listed ? sh.list_n : n;
-  auto value = [&](int i) { return listed ? sh.list_v[i] : at(i); };
-  const int seg = kBins / R;
-  auto histogram = [&](uint32_t lo, uint32_t hi, int shift) {
+  // ---- 4. many: thresholds by histograms, of what rank 0 has been given or of all slices
+  const int dn = local ? have : n;
+  auto value = [&](int i) { return local ? to_f32(given_v[i]) : at(i); };
+  auto reached = [&](bool by_count, u64 c, u64 f, uint32_t k_target, double p_target) {
+    return by_count ? c >= k_target : (double)f >= p_target;
+  };
+  // Entries with keys in [lo, hi] into bins of 2^shift keys from the top, and the bin in which the
+  // count (by_count) or the weight, from the sums above, reaches the target.
+  auto level = [&](uint32_t lo, uint32_t hi, int shift, bool by_count, const Found above, uint32_t k_target,
+                   double p_target) {
+    __syncthreads();
     for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = sh.m0[b] = sh.m1[b] = sh.m2[b] = 0;
+    if (tid == 0) sh.found = Found{-1, 0, 0, 0, 0};
     __syncthreads();
     for (int i = tid; i < dn; i += kSampThreads) {
       const float v = value(i);
-      const uint32_t kv = value_key(v);
+      const uint32_t kv = Key<T>::of(v);
       if (kv < lo || kv > hi) continue;
       const u64 f = fixed(weight(v));
       if (!f) continue;
@@ -437,62 +464,89 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
       atomicAdd(&sh.m1[b], (uint32_t)(f >> 15) & 0x7FFF);
       atomicAdd(&sh.m2[b], (uint32_t)(f >> 30));
     }
+    if (local) {
+      __syncthreads();
+      u64 c[2], f[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int b = 2 * tid + e;
+        c[e] = sh.count[b];
+        f[e] = (u64)sh.m0[b] + ((u64)sh.m1[b] << 15) + ((u64)sh.m2[b] << 30);
+      }
+      u64 ci = block_inclusive(c[0] + c[1], sh.warp_sum) + above.above - c[0] - c[1];
+      u64 fi = block_inclusive(f[0] + f[1], sh.warp_sum) + above.mass_above - f[0] - f[1];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {  // one bin of one thread is the first to reach the target
+        if (c[e] && reached(by_count, ci + c[e], fi + f[e], k_target, p_target) &&
+            ((ci == above.above && fi == above.mass_above) || !reached(by_count, ci, fi, k_target, p_target)))
+          sh.found = Found{2 * tid + e, (uint32_t)c[e], (uint32_t)ci, fi, f[e]};
+        ci += c[e];
+        fi += f[e];
+      }
+      __syncthreads();
+      return sh.found;
+    }
+    const int seg = kBins / R;
     cl.sync();
-    u64 cs = 0, ms = 0;
-    for (int b = tid; b < seg; b += kSampThreads) {
+    for (int i = tid; i < 4 * seg; i += kSampThreads) {  // four threads a bin, each some of the CTAs
+      const int g = rank * seg + (i >> 2);
       uint32_t c = 0;
       u64 f = 0;
 #pragma unroll 4
-      for (int r = 0; r < R; r++) {
+      for (int r = i & 3; r < R; r += 4) {
         const SampleShared* o = of(r);
-        const int g = rank * seg + b;
         c += o->count[g];
         f += (u64)o->m0[g] + ((u64)o->m1[g] << 15) + ((u64)o->m2[g] << 30);
       }
-      sh.seg_count[b] = c;
-      sh.seg_mass[b] = f;
-      cs += c;
-      ms += f;
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        c += __shfl_xor_sync(kFull, c, o);
+        f += __shfl_xor_sync(kFull, f, o);
+      }
+      if ((i & 3) == 0) {
+        sh.bin_count[i >> 2] = c;
+        sh.bin_mass[i >> 2] = f;
+      }
     }
-    cs = block_sum(cs, sh.warp_sum);
-    ms = block_sum(ms, sh.warp_sum);
-    if (tid == 0) {
-      sh.seg_count_sum = (uint32_t)cs;
-      sh.seg_mass_sum = ms;
-    }
-    cl.sync();
-  };
-  // the bin in which the count (by_count) or the weight reaches the target, from the sums above
-  auto find = [&](bool by_count, const Found& above, uint32_t k_target, double p_target) {
     __syncthreads();
     if (tid < 32) {
-      auto reached = [&](u64 cc, u64 ff) { return by_count ? cc >= k_target : (double)ff >= p_target; };
-      const u64 c0 = lane < R ? of(lane)->seg_count_sum : 0, f0 = lane < R ? of(lane)->seg_mass_sum : 0;
+      u64 cs = 0, ms = 0;
+      for (int b = lane; b < seg; b += 32) {
+        cs += sh.bin_count[b];
+        ms += sh.bin_mass[b];
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        cs += __shfl_xor_sync(kFull, cs, o);
+        ms += __shfl_xor_sync(kFull, ms, o);
+      }
+      if (lane == 0) {
+        sh.seg_count = (uint32_t)cs;
+        sh.seg_mass = ms;
+      }
+    }
+    cl.sync();
+    if (tid < 32) {
+      const u64 c0 = lane < R ? of(lane)->seg_count : 0, f0 = lane < R ? of(lane)->seg_mass : 0;
       const u64 ci = warp_inclusive(c0) + above.above, fi = warp_inclusive(f0) + above.mass_above;
-      const unsigned in = __ballot_sync(kFull, lane < R && c0 > 0 && reached(ci, fi));
-      Found f{-1, 0, 0, 0, 0};
+      const unsigned in = __ballot_sync(kFull, lane < R && c0 > 0 && reached(by_count, ci, fi, k_target, p_target));
       if (in) {
         const int r = __ffs(in) - 1;
         u64 c = __shfl_sync(kFull, ci - c0, r), g = __shfl_sync(kFull, fi - f0, r);
         const SampleShared* o = of(r);
         for (int b = 0; b < seg; b += 32) {  // 32 bins at a time
-          const u64 bc = b + lane < seg ? o->seg_count[b + lane] : 0, bf = b + lane < seg ? o->seg_mass[b + lane] : 0;
+          const u64 bc = o->bin_count[b + lane], bf = o->bin_mass[b + lane];
           const u64 ic = warp_inclusive(bc) + c, jf = warp_inclusive(bf) + g;
-          const unsigned hit = __ballot_sync(kFull, bc > 0 && reached(ic, jf));
+          const unsigned hit = __ballot_sync(kFull, bc > 0 && reached(by_count, ic, jf, k_target, p_target));
           if (hit) {
-            const int x = __ffs(hit) - 1;
-            f.bin = r * seg + b + x;
-            f.count = (uint32_t)__shfl_sync(kFull, bc, x);
-            f.mass = __shfl_sync(kFull, bf, x);
-            f.above = (uint32_t)__shfl_sync(kFull, ic - bc, x);
-            f.mass_above = __shfl_sync(kFull, jf - bf, x);
+            if (lane == __ffs(hit) - 1)
+              sh.found = Found{r * seg + b + lane, (uint32_t)bc, (uint32_t)(ic - bc), jf - bf, bf};
             break;
           }
           c = __shfl_sync(kFull, ic, 31);
           g = __shfl_sync(kFull, jf, 31);
         }
       }
-      if (tid == 0) sh.found = f;
     }
     __syncthreads();
     return sh.found;
@@ -500,18 +554,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   // the value in which the target is reached: its key, the sums above it and its own (bin -1: not
   // reached in the domain)
   auto select = [&](bool by_count, uint32_t k_target, double p_target, uint32_t* key) {
-    uint32_t hi = key_max, lo = 1;
-    if (last_step < kBins) {  // nothing of the domain is below this step's end
-      const float low = m - (float)(last_step + 1) / per_step * temp;
-      const float slack = 1e-5f * (fabsf(m) + fabsf(low)) + 1e-30f;
-      if (low - slack <= m) lo = max(1u, value_key(low - slack));
-    }
+    uint32_t hi = key_max, lo = max(1u, Key<T>::of(cut));
     Found f{0, 0, 0, 0, 0};
     for (;;) {
       int shift = 0;
       while (((hi - lo) >> shift) >= (uint32_t)kBins) shift++;
-      histogram(lo, hi, shift);
-      f = find(by_count, f, k_target, p_target);
+      f = level(lo, hi, shift, by_count, f, k_target, p_target);
       if (f.bin < 0) return f;
       const uint32_t top = hi - ((uint32_t)f.bin << shift);
       if (shift == 0) {
@@ -530,36 +578,35 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     if (f.bin >= 0) {
       ties = (uint32_t)k - f.above;
       mass = f.mass_above + f.mass / f.count * ties;
-    } else {  // fewer than k have any weight: the list holds all of them
-      by_k = false;
+    } else {  // fewer than k have any weight: top-k ends nothing, and they are all in the domain
+      key_t = 0;
       u64 mine = 0;
       for (int i = tid; i < dn; i += kSampThreads) mine += fixed(weight(value(i)));
       mine = block_sum(mine, sh.warp_sum);
       if (tid == 0) sh.exchange[0] = mine;
-      cl.sync();
-      mass = over_cluster(0);
+      if (local) {
+        mass = mine;
+      } else {
+        cl.sync();
+        mass = over_cluster(0);
+      }
     }
   }
   if (by_p) {
     const double target = (double)top_p * (double)mass;
-    if (!(target > 0.0)) {
-      key_t = key_max;
-      ties = 1;
-    } else {
-      uint32_t key_p = 0;
-      const Found f = select(false, 0, target, &key_p);
-      if (f.bin >= 0) {
-        const u64 each = f.mass / f.count;
-        // the fewest of the class that reach the target
-        u64 c = (double)f.mass_above >= target ? 1 : (u64)((target - (double)f.mass_above) / (double)each);
-        while (c > 1 && (double)(f.mass_above + (c - 1) * each) >= target) c--;
-        while (c < f.count && (double)(f.mass_above + c * each) < target) c++;
-        const uint32_t ties_p = (uint32_t)max((u64)1, c);
-        // the shorter of the two prefixes
-        if (key_p > key_t || (key_p == key_t && ties_p < ties)) {
-          key_t = key_p;
-          ties = ties_p;
-        }
+    uint32_t key_p = 0;
+    const Found f = select(false, 0, target, &key_p);
+    if (f.bin >= 0) {
+      const u64 each_f = f.mass / f.count;
+      // the fewest of the class that reach the target
+      u64 c = (double)f.mass_above >= target ? 1 : (u64)((target - (double)f.mass_above) / (double)each_f);
+      while (c > 1 && (double)(f.mass_above + (c - 1) * each_f) >= target) c--;
+      while (c < f.count && (double)(f.mass_above + c * each_f) < target) c++;
+      const uint32_t ties_p = (uint32_t)max((u64)1, c);
+      // the shorter of the two prefixes
+      if (key_p > key_t || (key_p == key_t && ties_p < ties)) {
+        key_t = key_p;
+        ties = ties_p;
       }
     }
   }
@@ -570,14 +617,17 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   uint32_t before = 0;  // entries equal to the threshold at lower indices
   if (ties != 0xFFFFFFFFu) {
     uint32_t mine = 0;
-    for (int i = d0; i < d1; i++) mine += value_key(value(i)) == key_t;
+    for (int i = d0; i < d1; i++) mine += Key<T>::of(value(i)) == key_t;
     const u64 incl = block_inclusive(mine, sh.warp_sum);
-    if (tid == kSampThreads - 1) sh.exchange[3] = incl;
-    cl.sync();
-    before = (uint32_t)(incl - mine + below_rank(3));
+    before = (uint32_t)(incl - mine);
+    if (!local) {
+      if (tid == kSampThreads - 1) sh.exchange[2] = incl;
+      cl.sync();
+      before += (uint32_t)below_rank(2);
+    }
   }
   auto kept = [&](float v, uint32_t& tie) -> u64 {
-    const uint32_t kv = value_key(v);
+    const uint32_t kv = Key<T>::of(v);
     if (kv < key_t) return 0;
     if (kv == key_t && tie++ >= ties) return 0;
     const float w = weight(v);
@@ -589,13 +639,19 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     for (int i = d0; i < d1; i++) mine += kept(value(i), tie);
   }
   u64 incl = block_inclusive(mine, sh.warp_sum);
-  if (tid == kSampThreads - 1) sh.exchange[2] = incl;
-  cl.sync();
-  const u64 total = over_cluster(2);
-  incl += below_rank(2);
+  if (tid == kSampThreads - 1) sh.exchange[3] = incl;
+  u64 total;
+  if (local) {
+    __syncthreads();
+    total = sh.exchange[3];
+  } else {
+    cl.sync();
+    total = over_cluster(3);
+    incl += below_rank(3);
+  }
   const double target = (double)u * (double)total;
   auto passed = [&](u64 c) { return (double)c > target || c >= total; };
-  if (mine && passed(incl) && !(incl - mine > 0 && passed(incl - mine))) {  // one thread of the cluster
+  if (mine && passed(incl) && !(incl - mine > 0 && passed(incl - mine))) {  // one thread
     u64 run = incl - mine;
     uint32_t tie = before;
     for (int i = d0; i < d1; i++) {
@@ -603,12 +659,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
       const u64 f = kept(v, tie);
       run += f;
       if (f && passed(run)) {
-        finish(listed ? sh.list_i[i] : base + i, weight(v), total);
+        finish(local ? given_i[i] : base + i, weight(v), total);
         break;
       }
     }
   }
-  cl.sync();  // no CTA leaves while others read its shared memory
+  if (!local) cl.sync();  // no CTA leaves while others read its shared memory
 }
 
 template <typename T>
@@ -625,6 +681,8 @@ cudaError_t launch(const SampleArgs& args, cudaStream_t s) {
   const size_t room = 200 * 1024 - head;
   a.cached = (int)std::min((size_t)a.slice, room / sizeof(T) / align * align);
   const size_t smem = head + (size_t)a.cached * sizeof(T);
+  a.given = (int)((size_t)a.cached * sizeof(T) / (sizeof(T) + 4)) / 8 * 8;
+  a.given_i = (int)(head + (size_t)a.given * sizeof(T));
   static bool wide[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -653,7 +711,7 @@ cudaError_t launch(const SampleArgs& args, cudaStream_t s) {
 cudaError_t launch_sample_rows(const void* logits, int dtype, int64_t row_stride, int rows, int vocab, const float* u,
                                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                                int32_t* ids, float* probs, cudaStream_t s) {
-  const SampleArgs a{logits, row_stride, rows, vocab, 0, 0, u, temperature, top_k, top_p, min_p, ids, probs};
+  const SampleArgs a{logits, row_stride, rows, vocab, 0, 0, 0, 0, u, temperature, top_k, top_p, min_p, ids, probs};
   if (dtype == DPUF_TYPE_F32) return launch<float>(a, s);
   if (dtype == DPUF_TYPE_F16) return launch<__half>(a, s);
   return launch<__nv_bfloat16>(a, s);

@@ -56,17 +56,24 @@ def _lib():
     return _typed
 
 
+# torch.cuda.current_stream() and current_device() build objects; these return the numbers
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+_raw_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 def _call(fn, device: int, *args) -> None:
     """Calls fn(*args, current stream) with `device` current."""
-    if torch.cuda.current_device() != device:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if _raw_device() == device:
+        rc = fn(*args, _raw_stream(device))
     else:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc == 0:
+        return
     if rc == -1:
         raise ValueError(engine.last_error())
-    if rc != 0:
-        raise RuntimeError(f"rc={rc}: {engine.last_error()}")
+    raise RuntimeError(f"rc={rc}: {engine.last_error()}")
 
 
 def _check(t: torch.Tensor, name: str, dtype, device: int, dims: int) -> None:
@@ -79,12 +86,13 @@ def _check(t: torch.Tensor, name: str, dtype, device: int, dims: int) -> None:
 
 
 def _check_table(t: torch.Tensor, device: int) -> None:
+    if t.dtype is _INT and t.get_device() == device and t.dim() == 2 and t.stride(1) == 1:
+        return
     if t.dtype != _INT:
         raise TypeError(f"page_table must be {_INT}, not {t.dtype}")
     if t.get_device() != device:
         raise ValueError(f"page_table must be on cuda:{device}")
-    if t.dim() != 2 or t.stride(1) != 1:
-        raise ValueError("page_table must be [sequences, pages] with neighbouring entries of a row adjacent")
+    raise ValueError("page_table must be [sequences, pages] with neighbouring entries of a row adjacent")
 
 
 class PagedCache:
@@ -192,17 +200,19 @@ def rope_append(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor, k:
         raise ValueError("the last dimension of q, k and v must be contiguous")
     if q.get_device() != dev or k.get_device() != dev or v.get_device() != dev:
         raise ValueError(f"q, k and v must be on cuda:{dev}")
-    _check(cos, "cos", _FLOAT, dev, 2)
-    _check(sin, "sin", _FLOAT, dev, 2)
-    _check(seq, "seq", _INT, dev, 1)
-    _check(pos, "pos", _INT, dev, 1)
-    _check_table(page_table, dev)
-    if cos.shape != sin.shape:
+    if not (cos.dtype is sin.dtype is _FLOAT and cos.get_device() == sin.get_device() == dev and cos.dim() == 2
+            and cos.is_contiguous() and sin.is_contiguous() and cos.shape == sin.shape):
+        _check(cos, "cos", _FLOAT, dev, 2)
+        _check(sin, "sin", _FLOAT, dev, 2)
         raise ValueError("cos and sin must have one shape")
-    if seq.shape[0] != n or pos.shape[0] != n:
+    if not (seq.dtype is pos.dtype is _INT and seq.get_device() == pos.get_device() == dev and seq.is_contiguous()
+            and pos.is_contiguous() and seq.shape == pos.shape == (n,)):
+        _check(seq, "seq", _INT, dev, 1)
+        _check(pos, "pos", _INT, dev, 1)
         raise ValueError("seq and pos must have one entry a token")
+    _check_table(page_table, dev)
     if out is None:
-        out = torch.empty((n, n_q, hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, n_q, hd))
     elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, of q's shape and on its device")
     elif out.dtype not in _CODE:
@@ -217,16 +227,17 @@ def rope_append(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor, k:
     return out
 
 
-def _workspace(device: int) -> torch.Tensor:
-    """The current stream's workspace: calls on one stream follow each other, so they can share it."""
-    key = (device, torch.cuda.current_stream(device).cuda_stream)
-    ws = _workspaces.get(key)
-    if ws is None:
+def _workspace(device: int) -> tuple:
+    """The current stream's workspace (tensor, address, bytes): calls on one stream follow each other, so they can share it."""
+    key = (device, _raw_stream(device))
+    found = _workspaces.get(key)
+    if found is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call paged_attention once on this stream before capturing it")
         n = _lib().dpuf_cuda_paged_attention_workspace()
-        ws = _workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=f"cuda:{device}")
-    return ws
+        ws = torch.zeros(n, dtype=torch.uint8, device=f"cuda:{device}")
+        found = _workspaces[key] = (ws, ws.data_ptr(), n)
+    return found
 
 
 def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor, q_start: torch.Tensor,
@@ -254,22 +265,24 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
         raise ValueError("the last dimension of q must be contiguous")
     if q.get_device() != dev:
         raise ValueError(f"q must be on cuda:{dev}")
-    _check(q_start, "q_start", _INT, dev, 1)
-    _check(kv_len, "kv_len", _INT, dev, 1)
     _check_table(page_table, dev)
     n_seqs, width = page_table.shape
-    if q_start.shape[0] != n_seqs + 1 or kv_len.shape[0] != n_seqs:
+    if not (q_start.dtype is kv_len.dtype is _INT and q_start.get_device() == kv_len.get_device() == dev
+            and q_start.is_contiguous() and kv_len.is_contiguous() and q_start.shape == (n_seqs + 1,)
+            and kv_len.shape == (n_seqs,)):
+        _check(q_start, "q_start", _INT, dev, 1)
+        _check(kv_len, "kv_len", _INT, dev, 1)
         raise ValueError("q_start must have one entry more than page_table has rows, kv_len as many")
     if out is None:
-        out = torch.empty((n, n_q, hd), dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, n_q, hd))
     elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, of q's shape and on its device")
     elif out.dtype != q.dtype and out.dtype != _FLOAT:
         raise TypeError("out must be float32 or of q's type")
-    ws = _workspace(dev)
+    _, ws, ws_bytes = _workspace(dev)
     args = cache._packed + _ATTN.pack(
         page_table.data_ptr(), page_table.stride(0), q.data_ptr(), qs[0], qs[1], out.data_ptr(), q_start.data_ptr(),
-        kv_len.data_ptr(), ws.data_ptr(), ws.numel(), n_seqs, width, n, n_q, max_q, bool(causal), window, code,
+        kv_len.data_ptr(), ws, ws_bytes, n_seqs, width, n, n_q, max_q, bool(causal), window, code,
         _CODE[out.dtype], hd ** -0.5 if scale is None else scale)
     _call(_lib().dpuf_cuda_paged_attention, dev, args)
     return out
@@ -279,7 +292,7 @@ def attention_check(device: int | None = None) -> None:
     """Waits for the current stream and raises RuntimeError if a bounded wait inside one of its
     `paged_attention` calls gave up since the last check (that call's output is undefined)."""
     dev = torch.cuda.current_device() if device is None else device
-    _call(_lib().dpuf_cuda_paged_attention_status, dev, _workspace(dev).data_ptr())
+    _call(_lib().dpuf_cuda_paged_attention_status, dev, _workspace(dev)[1])
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None,
@@ -302,17 +315,21 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | No
         raise ValueError("logits must be on a GPU")
     dev = logits.get_device()
     rows, vocab = logits.shape
-    for t, name, dtype in ((u, "u", _FLOAT), (temperature, "temperature", _FLOAT), (top_k, "top_k", _INT),
-                           (top_p, "top_p", _FLOAT), (min_p, "min_p", _FLOAT)):
+    if u is None:
+        raise TypeError("u is needed")
+
+    def row_values(t, name, dtype):
         if t is None:
-            if name == "u":
-                raise TypeError("u is needed")
-            continue
-        _check(t, name, dtype, dev, 1)
-        if t.shape[0] != rows:
+            return None
+        if not (t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.shape == (rows,)):
+            _check(t, name, dtype, dev, 1)
             raise ValueError(f"{name} must have one entry a row")
-    ids = torch.empty(rows, dtype=_INT, device=logits.device)
-    probs = torch.empty(rows, dtype=_FLOAT, device=logits.device)
-    ptr = [None if t is None else t.data_ptr() for t in (u, temperature, top_k, top_p, min_p, ids, probs)]
-    _call(_lib().dpuf_cuda_sample_rows, dev, logits.data_ptr(), code, logits.stride(0), rows, vocab, *ptr)
+        return t.data_ptr()
+
+    values = (row_values(u, "u", _FLOAT), row_values(temperature, "temperature", _FLOAT),
+              row_values(top_k, "top_k", _INT), row_values(top_p, "top_p", _FLOAT), row_values(min_p, "min_p", _FLOAT))
+    probs = u.new_empty(rows)
+    ids = probs.new_empty(rows, dtype=_INT)
+    _call(_lib().dpuf_cuda_sample_rows, dev, logits.data_ptr(), code, logits.stride(0), rows, vocab,
+          *values, ids.data_ptr(), probs.data_ptr())
     return ids, probs
