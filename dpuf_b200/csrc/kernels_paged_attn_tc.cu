@@ -1,28 +1,29 @@
 // kernels_paged_attn_tc.cu - attention of chunks of new tokens over the paged cache on the
 // 5th-generation tensor cores (tcgen05, TMEM), 16-bit queries and cache, head_dim <= 128.
 //
-// An item is 256 rows of one sequence and KV head (two tiles of 128), walked in blocks of 128
-// keys; per tile and block S = Q K^T (M = 128, N = 128) into TMEM, the softmax's weights P from S
-// with the running maximum and sum (kernels_paged_attn.cu has the formulas), O += P V with P read
-// from TMEM.  Two tiles share the keys and values, and while one's softmax runs on the CUDA cores
-// the other's products run on the tensor cores.
+// An item is 256 rows of one sequence and KV head (two tiles of 128), walked in blocks of 64 keys;
+// per tile and block S = Q K^T (M = 128, N = 64) into TMEM, the softmax's weights P from S with the
+// running maximum and sum (kernels_paged_attn.cu has the formulas), O += P V with P read from TMEM.
 //
-//   warps 0..3, 4..7  softmax of tile 0, 1: a thread has one row.  It reads its 128 scores, writes
-//                     P (rounded to the cache's type; the sum keeps the unrounded weights) over
-//                     them, and scales O in TMEM only when its row's maximum has grown by more
-//                     than 2^8 since the last time (weights are then at most 2^8, which both types
-//                     hold with their full precision; the division by the sum at the end makes up
-//                     for it), which after the first blocks is rare.
+//   warps 0..3, 4..7  softmax of tile 0, 1: a thread has one row.  It reads its 64 scores, writes P
+//                     (rounded to the cache's type; the sum keeps the unrounded weights) over them,
+//                     and scales O in TMEM only when its row's maximum has grown by more than 2^8
+//                     since the last time (weights are then at most 2^8, which both types hold with
+//                     their full precision; the division by the sum at the end makes up for it),
+//                     which after the first blocks is rare.
 //   warp 8            TMA: 64-column boxes of a page's rows (128-byte swizzle) into a ring of key
 //                     and value blocks; a page that is not held, or that no row sees, is a box
 //                     outside the tensor and arrives as zeros.
-//   warp 9            issues the MMAs of whichever tile is ready, each tile's products in turn;
+//   warp 9            issues the MMAs of whichever tile is ready, weights' products before scores;
 //                     zeroes the rows of a value block that no row of the item sees (stale cache
 //                     contents may be infinite or NaN, and 0 times those is NaN; scores of such
 //                     keys are replaced, not multiplied).
 //
-// TMEM: S0, S1 (128 columns each; P in the first 64), O0, O1.  A tile's next S may only be
-// written once its P has been read, so the QK of block b + 1 waits for the PV of block b.
+// TMEM: each tile has two score buffers of 64 columns (P in the first 32 of each) and O; all 512
+// columns.  The second buffer is what the 64-key block buys: the next block's scores are computed
+// while the softmax works on this one's.  With one buffer of 128 (P over S, so that QK waits for
+// PV and the softmax for both) neither unit was busy half of the time.  The price: at N = 64 the
+// QK reads 6 KB of shared memory per 32 tensor cycles, 1.5 times what it delivers.
 //
 // Every wait is bounded: one that gives up sets the workspace's error word and the CTA's abort
 // flag, all roles stop, copies in flight are waited for (bounded) and TMEM is freed.
@@ -36,7 +37,8 @@ namespace dpuf {
 
 namespace {
 
-constexpr int kTile = 128;            // rows of a tile, keys of a block
+constexpr int kTile = 128;            // rows of a tile
+constexpr int kKeys = 64;             // of a block
 constexpr int kItemRows = 2 * kTile;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 320;
@@ -61,6 +63,14 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n, int b_mn) {
          ((uint32_t)(kTile >> 4) << 24);
 }
 
+// One lane of the warp, the same each time.  The compiler then knows that a single thread issues
+// what follows (with a test of the lane it does not, and wraps each MMA in a loop over lanes:
+// 700 cycles instead of 400 to 500 for the eight of a product).
+DPUF_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+  return p != 0;
+}
 DPUF_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -104,19 +114,22 @@ DPUF_DEV void tmem_st32(uint32_t addr, const uint32_t* v) {
       "r"(addr)
       : "memory");
 }
-// 8 columns, there on return.
-DPUF_DEV void tmem_ld8(uint32_t addr, uint32_t* v) {
+// 16 columns, there on return.
+DPUF_DEV void tmem_ld16(uint32_t addr, uint32_t* v) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(addr)
       : "memory");
 }
-DPUF_DEV void tmem_st8(uint32_t addr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]),
-               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
-               : "memory");
+DPUF_DEV void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+      "%14, %15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
+      : "memory");
 }
 DPUF_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 DPUF_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -187,19 +200,20 @@ DPUF_DEV uint32_t pack2(float a, float b, __nv_bfloat16) {
 }
 
 template <int DP>
-struct TileLay {  // shared memory, from a 1,024-byte boundary
-  static constexpr int stages = DP == 128 ? 2 : 4;
-  static constexpr int block = kTile * DP * 2;  // 64-column runs of [128][128 bytes]
-  static constexpr int q = 0;                   // [2][block]
-  static constexpr int k = q + 2 * block;       // [stages][block]
+struct TileLay {  // shared memory, from a 1,024-byte boundary; operands are 64-column runs of [rows][128 bytes]
+  static constexpr int stages = DP == 128 ? 4 : 6;
+  static constexpr int tile = kTile * DP * 2;
+  static constexpr int block = kKeys * DP * 2;
+  static constexpr int q = 0;                   // [2][tile]
+  static constexpr int k = q + 2 * tile;        // [stages][block]
   static constexpr int v = k + stages * block;  // [stages][block]
   static constexpr int bytes = v + stages * block + 1024;
 };
-constexpr int kRun = kTile * 128;  // bytes of a 64-column run
+constexpr int kQRun = kTile * 128, kKvRun = kKeys * 128;  // bytes of a 64-column run
 
 struct TileArgs {
   AttnArgs p;
-  CUtensorMap k_map, v_map;  // (dim, row, head, page), boxes of 64 x min(page_size, 128)
+  CUtensorMap k_map, v_map;  // (dim, row, head, page), boxes of 64 x min(page_size, 64)
 };
 
 // Positions that an item's rows [r0, r0 + rows) see between them.
@@ -213,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
   constexpr int S = Lay::stages;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S];
-  __shared__ __align__(8) uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+  __shared__ __align__(8) uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2];
   __shared__ AttnShare share;
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_sh, flag_sh[2];
@@ -236,15 +250,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     }
     for (int i = 0; i < 2; i++) {
       bar_init(&q_full[i], kTile);
-      bar_init(&s_full[i], 1);
-      bar_init(&p_full[i], kTile);
-      bar_init(&pv_done[i], 1);
+      for (int h = 0; h < 2; h++) {
+        bar_init(&s_full[i][h], 1);
+        bar_init(&p_full[i][h], kTile);
+        bar_init(&pv_done[i][h], 1);
+      }
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     abort_sh = 0;
   }
   fence_before();
-  AttnRun run = attn_locate<kItemRows, kTile>(p, share, blockIdx.x, gridDim.x);
+  AttnRun run = attn_locate<kItemRows, kKeys>(p, share, blockIdx.x, gridDim.x);
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_sh;
@@ -252,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
 
   if (warp == kLoadWarp) {
     // ================================================================ TMA
-    const int box = min(p.a.kv.page_size, kTile), boxes = kTile / box;
+    const int box = min(p.a.kv.page_size, kKeys), boxes = kKeys / box;
     unsigned it = 0;  // blocks requested so far
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
@@ -261,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       int lo, hi;
       item_span(p, c.seq, c.tile, &lo, &hi);
       auto page_of = [&](int b) {  // of this lane's box
-        const int j = (c.blk0 + b) * kTile + lane * box;
+        const int j = (c.blk0 + b) * kKeys + lane * box;
         int page = p.a.kv.n_pages;  // outside the tensor
         if (lane < boxes && j < hi && j + box > lo) {
           page = p.a.page_table[(size_t)c.s * p.a.table_stride + (j >> p.page_shift)];
@@ -274,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         const int next = b + 1 < to ? page_of(b + 1) : 0;
         const int slot = it % S;
         const unsigned par = (it / S & 1) ^ 1;
-        const int row = ((c.blk0 + b) * kTile + lane * box) & (p.a.kv.page_size - 1);
+        const int row = ((c.blk0 + b) * kKeys + lane * box) & (p.a.kv.page_size - 1);
         auto copy = [&](const CUtensorMap* map, uint64_t* full, unsigned char* dst) {
           if (lane == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(full)), "r"(Lay::block)
@@ -285,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
             for (int h = 0; h < DP / 64; h++)
               asm volatile(
                   "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-                  "%3, %4, %5}], [%6];" ::"r"(su32(dst + h * kRun + lane * box * 128)),
+                  "%3, %4, %5}], [%6];" ::"r"(su32(dst + h * kKvRun + lane * box * 128)),
                   "l"(map), "r"(h * 64), "r"(row), "r"(c.head), "r"(page), "r"(su32(full))
                   : "memory");
         };
@@ -298,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         copy(&args.v_map, &v_full[slot], sm + Lay::v + slot * Lay::block);
         page = next;
       }
-      if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
     }
     if (!ok)  // nothing in flight at exit (waits of at most 2 s each; a value block may be missing)
       for (unsigned i = it > S ? it - S : 0; i < it; i++) {
@@ -309,9 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       }
   } else if (warp == kMmaWarp) {
     // ================================================================ MMA
-    constexpr uint32_t kIdQk = idesc_f16<T>(kTile, 0), kIdPv = idesc_f16<T>(DP, 1);
-    unsigned base = 0;                     // blocks of earlier items
-    unsigned items[2] = {0, 0};            // items and blocks of each tile so far
+    constexpr uint32_t kIdQk = idesc_f16<T>(kKeys, 0), kIdPv = idesc_f16<T>(DP, 1);
+    unsigned base = 0;             // blocks of earlier items
+    unsigned items[2] = {0, 0};    // items and blocks of each tile so far
     unsigned blocks[2] = {0, 0};
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
@@ -320,71 +336,71 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       int lo, hi;
       item_span(p, c.seq, c.tile, &lo, &hi);
       const int tiles = c.seq.qn * p.group - c.tile * kItemRows > kTile ? 2 : 1;
-      int qk[2] = {0, 0}, pv[2] = {0, 0}, cleaned = -1;
+      int qk[2] = {0, 0}, pv[2] = {0, 0}, cleaned = -1;  // products issued
       unsigned long long t0 = 0;
       for (int idle = 0;;) {
         bool moved = false;
-        for (int i = 0; i < tiles; i++) {
-          if (pv[i] == n) continue;
-          const bool want_qk = qk[i] == pv[i];
-          const int b = want_qk ? qk[i] : pv[i];
-          const unsigned g = base + b;
-          const int slot = g % S;
-          const unsigned par = g / S & 1;
-          if (want_qk) {
-            bool ready = bar_test(&k_full[slot], par);
-            if (b == 0) ready = ready && bar_test(&q_full[i], items[i] & 1);
-            if (blocks[i] > 0) ready = ready && bar_test(&pv_done[i], (blocks[i] - 1) & 1);
-            if (!__all_sync(kFull, ready)) continue;
-            if (lane == 0) {
-              fence_after();
-              const uint64_t da = sw128_desc(sm + Lay::q + i * Lay::block, 16, 1024);
-              const uint64_t db = sw128_desc(sm + Lay::k + slot * Lay::block, 16, 1024);
 #pragma unroll
-              for (int s = 0; s < DP / 16; s++) {  // 16 columns = 32 bytes a step
-                const uint64_t o = (uint64_t)((s / 4) * (kRun >> 4) + (s % 4) * 2);
-                mma_ss(tmem + i * kTile, da + o, db + o, kIdQk, s > 0);
+        for (int i = 0; i < 2; i++) {
+          if (i >= tiles) continue;
+          if (pv[i] < qk[i]) {  // weights that may be there
+            const int b = pv[i];
+            const unsigned g = base + b, e = blocks[i] + b;
+            const int slot = g % S;
+            if (__all_sync(kFull, bar_test(&p_full[i][e & 1], e >> 1 & 1) && bar_test(&v_full[slot], g / S & 1))) {
+              if (cleaned < b) {  // once per value block
+                cleaned = b;
+                const int j0 = (c.blk0 + from + b) * kKeys;
+                const int z0 = max(lo - j0, 0), z1 = min(hi - j0, kKeys);  // rows to keep
+                if (z0 > 0 || z1 < kKeys) {
+                  unsigned char* v = sm + Lay::v + slot * Lay::block;
+                  for (int r = lane >> 3; r < kKeys; r += 4)
+                    if (r < z0 || r >= z1)
+#pragma unroll
+                      for (int h = 0; h < DP / 64; h++)
+                        *(uint4*)(v + h * kKvRun + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                  __syncwarp();
+                }
               }
-              mma_commit(&s_full[i]);
-            }
-            qk[i]++;
-            if (tiles == 1 || qk[i ^ 1] > b) {
-              if (lane == 0) mma_commit(&k_empty[slot]);
-            }
-          } else {
-            bool ready = bar_test(&v_full[slot], par) && bar_test(&p_full[i], blocks[i] & 1);
-            if (!__all_sync(kFull, ready)) continue;
-            if (cleaned < b) {  // once per value block
-              cleaned = b;
-              const int j0 = (c.blk0 + from + b) * kTile;
-              const int z0 = max(lo - j0, 0), z1 = min(hi - j0, kTile);  // rows to keep
-              if (z0 > 0 || z1 < kTile) {
-                unsigned char* v = sm + Lay::v + slot * Lay::block;
-                for (int r = lane >> 3; r < kTile; r += 4)
-                  if (r < z0 || r >= z1)
+              pv[i]++;
+              if (elect_one()) {
+                fence_after();
+                const uint64_t db = sw128_desc(sm + Lay::v + slot * Lay::block, kKvRun, 1024);
+                const uint32_t a = tmem + i * kTile + (e & 1) * kKeys, d = tmem + 2 * kTile + i * kTile;
 #pragma unroll
-                    for (int h = 0; h < DP / 64; h++)
-                      *(uint4*)(v + h * kRun + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
+                for (int s = 0; s < kKeys / 16; s++)  // 16 keys = 2,048 bytes of V, 8 columns of P a step
+                  mma_ts(d, a + s * 8, db + (uint64_t)(s * 128), kIdPv, b > 0 || s > 0);
+                mma_commit(&pv_done[i][e & 1]);
+                if (tiles == 1 || pv[i ^ 1] > b) mma_commit(&v_empty[slot]);
               }
-            }
-            if (lane == 0) {
-              fence_after();
-              const uint64_t db = sw128_desc(sm + Lay::v + slot * Lay::block, kRun, 1024);
-#pragma unroll
-              for (int s = 0; s < kTile / 16; s++)  // 16 keys = 2,048 bytes of V, 8 columns of P a step
-                mma_ts(tmem + 2 * kTile + i * kTile, tmem + i * kTile + s * 8, db + (uint64_t)(s * 128), kIdPv,
-                       b > 0 || s > 0);
-              mma_commit(&pv_done[i]);
-            }
-            pv[i]++;
-            blocks[i]++;
-            if (tiles == 1 || pv[i ^ 1] > b) {
-              if (lane == 0) mma_commit(&v_empty[slot]);
+              moved = true;
             }
           }
-          moved = true;
+          if (qk[i] < n && qk[i] < pv[i] + 2) {  // scores: their buffer's earlier weights have been read
+            const int b = qk[i];
+            const unsigned g = base + b, e = blocks[i] + b;
+            const int slot = g % S;
+            bool ready = bar_test(&k_full[slot], g / S & 1);
+            if (b == 0) ready = ready && bar_test(&q_full[i], items[i] & 1);
+            if (e >= 2) ready = ready && bar_test(&pv_done[i][e & 1], (e - 2) >> 1 & 1);
+            if (__all_sync(kFull, ready)) {
+              qk[i]++;
+              if (elect_one()) {
+                fence_after();
+                const uint64_t da = sw128_desc(sm + Lay::q + i * Lay::tile, 16, 1024);
+                const uint64_t db = sw128_desc(sm + Lay::k + slot * Lay::block, 16, 1024);
+                const uint32_t d = tmem + i * kTile + (e & 1) * kKeys;
+#pragma unroll
+                for (int s = 0; s < DP / 16; s++)  // 16 columns = 32 bytes a step
+                  mma_ss(d, da + (uint64_t)((s / 4) * (kQRun >> 4) + (s % 4) * 2),
+                         db + (uint64_t)((s / 4) * (kKvRun >> 4) + (s % 4) * 2), kIdQk, s > 0);
+                mma_commit(&s_full[i][e & 1]);
+                if (tiles == 1 || qk[i ^ 1] > b) mma_commit(&k_empty[slot]);
+              }
+              moved = true;
+            }
+          }
         }
         if (pv[0] == n && (tiles == 1 || pv[1] == n)) break;
         if (moved) {
@@ -392,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         } else if (++idle == 64) {
           t0 = gtimer();
         } else if (idle > 64 && (idle & 63) == 0) {
-          bool late = gtimer() - t0 > kWaitNs;
+          const bool late = gtimer() - t0 > kWaitNs;
           if (late) {
             *give.abort = 1;
             atomicCAS(give.err, 0, 1);
@@ -403,9 +419,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           }
         }
       }
-      for (int i = 0; i < tiles; i++) items[i]++;
+      for (int i = 0; i < tiles; i++) {
+        items[i]++;
+        blocks[i] += n;
+      }
       base += n;
-      if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
     }
   } else {
     // ================================================================ softmax: tile w, this thread's row
@@ -424,20 +443,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       left -= n;
       const int total = c.seq.qn * p.group, r0 = c.tile * kItemRows + w * kTile;
       if (w == 1 && r0 >= total) {  // one tile only
-        if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+        if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
         continue;
       }
       // ---- this tile's queries (the earlier item's products are complete: its last scores were)
-      unsigned char* qs = sm + Lay::q + w * Lay::block;
-      for (int i = t; i < kTile * (DP / 8); i += kTile) {
-        const int r = i / (DP / 8), ch = i % (DP / 8), rr = r0 + r;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (rr < total && ch * 8 < hd) {
-          x = *(const uint4*)((const T*)p.a.q + (int64_t)(c.seq.q0 + rr / p.group) * p.a.q_stride[0] +
-                              (int64_t)(c.head * p.group + rr % p.group) * p.a.q_stride[1] + ch * 8);
-          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+      unsigned char* qs = sm + Lay::q + w * Lay::tile;
+      {
+        constexpr int kCh = DP / 8, kStep = kTile / kCh, kBatch = 8;  // 16-byte chunks of a row, rows of a pass
+        const int ch = t % kCh;
+#pragma unroll 1
+        for (int k0 = 0; k0 < kCh; k0 += kBatch) {
+          uint4 x[kBatch];
+#pragma unroll
+          for (int k = 0; k < kBatch; k++) {  // loads of several passes in flight
+            const int rr = r0 + t / kCh + (k0 + k) * kStep;
+            x[k] = make_uint4(0, 0, 0, 0);
+            if (rr < total && ch * 8 < hd)
+              x[k] = __ldg((const uint4*)((const T*)p.a.q + (int64_t)(c.seq.q0 + rr / p.group) * p.a.q_stride[0] +
+                                          (int64_t)(c.head * p.group + rr % p.group) * p.a.q_stride[1] + ch * 8));
+          }
+#pragma unroll
+          for (int k = 0; k < kBatch; k++) {
+            const int r = t / kCh + (k0 + k) * kStep;
+            x[k].x ^= flip; x[k].y ^= flip; x[k].z ^= flip; x[k].w ^= flip;
+            *(uint4*)(qs + (ch >> 3) * kQRun + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[k];
+          }
         }
-        *(uint4*)(qs + (ch >> 3) * kRun + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_arrive(&q_full[w]);
@@ -448,24 +479,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       if (live) attn_span(p, c.seq, tok, tok, &lo, &hi);
       float m = -CUDART_INF_F, l = 0.0f;  // m: the maximum that the weights refer to
       for (int b = 0; b < n; b++, blocks++) {
-        const int j0 = (c.blk0 + from + b) * kTile;
-        if (!(ok = warp_wait(&s_full[w], blocks & 1, give))) break;
+        const int j0 = (c.blk0 + from + b) * kKeys, h = blocks & 1;
+        if (!(ok = warp_wait(&s_full[w][h], blocks >> 1 & 1, give))) break;
         fence_after();
-        uint32_t s[kTile];
-#pragma unroll
-        for (int i = 0; i < 4; i++) tmem_ld32(tS + 32 * i, s + 32 * i);
+        uint32_t s[kKeys];
+        tmem_ld32(tS + h * kKeys, s);
+        tmem_ld32(tS + h * kKeys + 32, s + 32);
         tmem_wait_ld();
-        if (!__all_sync(kFull, lo <= j0 && j0 + kTile <= hi)) {
+        if (!__all_sync(kFull, lo <= j0 && j0 + kKeys <= hi)) {
           const int a = lo - j0, e = hi - j0;
 #pragma unroll
-          for (int i = 0; i < kTile; i++)
+          for (int i = 0; i < kKeys; i++)
             if (i < a || i >= e) s[i] = 0xFF800000u;  // -inf
         }
         float t4[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) t4[i] = __uint_as_float(s[i]);
 #pragma unroll
-        for (int i = 4; i < kTile; i++) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(s[i]));
+        for (int i = 4; i < kKeys; i++) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(s[i]));
         const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
         const bool grow = b == 0 || m == -CUDART_INF_F ? top > m : (top - m) * sl > 8.0f;
         if (__any_sync(kFull, grow)) {
@@ -473,34 +504,35 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           const float f = !grow ? 1.0f : m == -CUDART_INF_F ? 0.0f : ex2((m - m2) * sl);
           l *= f;
           m = m2;
-          if (b > 0) {
+          if (b > 0) {  // O as the product of the block before leaves it
+            if (!(ok = warp_wait(&pv_done[w][h ^ 1], (blocks - 1) >> 1 & 1, give))) break;
+            fence_after();
 #pragma unroll 1
-            for (int i = 0; i < DP / 8; i++) {  // few columns at a time: the scores hold the registers
-              uint32_t o[8];
-              tmem_ld8(tO + 8 * i, o);
+            for (int i = 0; i < DP / 16; i++) {
+              uint32_t o[16];
+              tmem_ld16(tO + 16 * i, o);
 #pragma unroll
-              for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st8(tO + 8 * i, o);
+              for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(tO + 16 * i, o);
             }
           }
         }
         const float ref = m == -CUDART_INF_F ? 0.0f : __fmaf_rn(m, sl, -kLift);
         float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < kTile; i += 2) {
+        for (int i = 0; i < kKeys; i += 2) {
           const float a = ex2(__fmaf_rn(__uint_as_float(s[i]), sl, -ref));
           const float e = ex2(__fmaf_rn(__uint_as_float(s[i + 1]), sl, -ref));
           l4[i / 2 & 3] += a + e;
           s[i / 2] = pack2(a, e, T());
         }
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-        tmem_st32(tS, s);
-        tmem_st32(tS + 32, s + 32);
+        tmem_st32(tS + h * kKeys, s);
         tmem_wait_st();
         fence_before();
-        bar_arrive(&p_full[w]);
+        bar_arrive(&p_full[w][h]);
       }
-      if (!ok || !(ok = warp_wait(&pv_done[w], (blocks - 1) & 1, give))) break;
+      if (!ok || !(ok = warp_wait(&pv_done[w][(blocks - 1) & 1], (blocks - 1) >> 1 & 1, give))) break;
       fence_after();
 
       // ---- the whole item, or a part of it
@@ -543,38 +575,42 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
         const size_t at = ((size_t)(c.seq.q0 + tok) * p.a.n_q + head) * hd;
 #pragma unroll
-        for (int i = 0; i < DP / 32; i++) {
-          uint32_t o[32];
+        for (int i = 0; i < DP / 64; i++) {
+          uint32_t o[64];
           if (whole) {
-            tmem_ld32(tO + 32 * i, o);
+            tmem_ld32(tO + 64 * i, o);
+            tmem_ld32(tO + 64 * i + 32, o + 32);
             tmem_wait_ld();
           } else {
             const int pr = w * kTile + t;
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = 0;
+            for (int e = 0; e < 64; e++) o[e] = 0;
+#pragma unroll 1
             for (int cc = c0; cc <= c1; cc++) {
               const size_t slot = 2 * (size_t)cc + (cc == c0);
               const float x = __ldcg(&parts.ml[slot * kItemRows + pr]).x;
+              const float* src = parts.o + (slot * DP + 64 * i) * kItemRows + pr;
+              float y[64];
+#pragma unroll
+              for (int e = 0; e < 64; e++) y[e] = __ldcg(src + e * kItemRows);
               const float f = x == -CUDART_INF_F ? 0.0f : ex2(x - m);
 #pragma unroll
-              for (int e = 0; e < 32; e++)
-                o[e] = __float_as_uint(__fmaf_rn(__ldcg(&parts.o[(slot * DP + 32 * i + e) * kItemRows + pr]), f,
-                                                 __uint_as_float(o[e])));
+              for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__fmaf_rn(y[e], f, __uint_as_float(o[e])));
             }
           }
           if (live)
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-              if (32 * i + 8 * g < hd) {
+            for (int g = 0; g < 8; g++)
+              if (64 * i + 8 * g < hd) {
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[e] = __uint_as_float(o[8 * g + e]) * inv;
-                store8_as(p.a.out, at + 32 * i + 8 * g, p.a.out_dtype, x);
+                store8_as(p.a.out, at + 64 * i + 8 * g, p.a.out_dtype, x);
               }
         }
       }
       fence_before();  // O is read: the next item's products may overwrite it once its P arrives
-      if (left > 0) attn_next_item<kItemRows, kTile>(p, c);
+      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
     }
   }
   fence_before();
@@ -604,7 +640,7 @@ bool encode(CUtensorMap* map, const DpufPagedKv& kv, void* base) {
                               (cuuint64_t)kv.n_pages};
   const cuuint64_t strides[3] = {(cuuint64_t)kv.row_stride * 2, (cuuint64_t)kv.head_stride * 2,
                                  (cuuint64_t)kv.page_stride * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(kv.page_size, kTile), 1, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(kv.page_size, kKeys), 1, 1}, one[4] = {1, 1, 1, 1};
   return encoder()(map, kv.dtype == DPUF_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                    4, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
