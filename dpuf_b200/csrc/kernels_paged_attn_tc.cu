@@ -14,10 +14,10 @@
 //   warp 8            TMA: 64-column boxes of a page's rows (128-byte swizzle) into a ring of key
 //                     and value blocks; a page that is not held, or that no row sees, is a box
 //                     outside the tensor and arrives as zeros.
-//   warp 9            issues the MMAs of whichever tile is ready, weights' products before scores;
-//                     zeroes the rows of a value block that no row of the item sees (stale cache
-//                     contents may be infinite or NaN, and 0 times those is NaN; scores of such
-//                     keys are replaced, not multiplied).
+//   warps 9, 10       issue tile 0's and tile 1's MMAs (one warp for both was the limit: its waits
+//                     left the tensor cores idle); they zero the rows of a value block that no row
+//                     of the item sees (stale cache contents may be infinite or NaN, and 0 times
+//                     those is NaN; scores of such keys are replaced, not multiplied).
 //
 // TMEM: each tile has two score buffers of 64 columns (P in the first 32 of each) and O; all 512
 // columns.  The second buffer is what the 64-key block buys: the next block's scores are computed
@@ -40,8 +40,8 @@ namespace {
 constexpr int kTile = 128;            // rows of a tile
 constexpr int kKeys = 64;             // of a block
 constexpr int kItemRows = 2 * kTile;
-constexpr int kLoadWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 320;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;  // kMmaWarp + i: tile i
+constexpr int kThreads = 352;
 // The weights carry a factor 2^7, and so does their sum: at most 2^15, which fp16 holds, while the
 // small ones of a long context keep their bits.
 constexpr float kLift = 7.0f;
@@ -155,14 +155,6 @@ DPUF_DEV bool bar_try(uint64_t* bar, unsigned par) {
                : "memory");
   return ok != 0;
 }
-DPUF_DEV bool bar_test(uint64_t* bar, unsigned par) {
-  unsigned ok;
-  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-               : "=r"(ok)
-               : "r"(su32(bar)), "r"(par)
-               : "memory");
-  return ok != 0;
-}
 
 struct Give {  // where a wait that gives up says so
   volatile int* abort;
@@ -244,9 +236,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
   if (tid == 0) {
     for (int i = 0; i < S; i++) {
       bar_init(&k_full[i], 1);
-      bar_init(&k_empty[i], 1);
+      bar_init(&k_empty[i], 2);
       bar_init(&v_full[i], 1);
-      bar_init(&v_empty[i], 1);
+      bar_init(&v_empty[i], 2);
     }
     for (int i = 0; i < 2; i++) {
       bar_init(&q_full[i], kTile);
@@ -323,105 +315,83 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         const unsigned long long t1 = gtimer();
         while (!bar_try(&v_full[i % S], i / S & 1) && gtimer() - t1 < kWaitNs / 100) {}
       }
-  } else if (warp == kMmaWarp) {
-    // ================================================================ MMA
+  } else if (warp >= kMmaWarp) {
+    // ================================================================ MMA of tile w
     constexpr uint32_t kIdQk = idesc_f16<T>(kKeys, 0), kIdPv = idesc_f16<T>(DP, 1);
-    unsigned base = 0;             // blocks of earlier items
-    unsigned items[2] = {0, 0};    // items and blocks of each tile so far
-    unsigned blocks[2] = {0, 0};
+    const int w = warp - kMmaWarp;
+    const uint64_t dq = sw128_desc(sm + Lay::q + w * Lay::tile, 16, 1024);
+    const uint64_t dk = sw128_desc(sm + Lay::k, 16, 1024), dv = sw128_desc(sm + Lay::v, kKvRun, 1024);
+    const uint32_t ts = tmem + w * kTile, to_ = tmem + 2 * kTile + w * kTile;
+    unsigned base = 0;                // blocks of earlier items
+    unsigned items = 0, blocks = 0;   // of this tile so far
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
       const int from = c.at, to = min(c.n_blk, c.at + left), n = to - from;
       left -= n;
       int lo, hi;
       item_span(p, c.seq, c.tile, &lo, &hi);
-      const int tiles = c.seq.qn * p.group - c.tile * kItemRows > kTile ? 2 : 1;
-      int qk[2] = {0, 0}, pv[2] = {0, 0}, cleaned = -1;  // products issued
-      unsigned long long t0 = 0;
-      for (int idle = 0;;) {
-        bool moved = false;
+      const bool mine = w == 0 || c.seq.qn * p.group - c.tile * kItemRows > kTile;
+      // scores of block b into its buffer, whose earlier weights have been read
+      auto scores = [&](int b) {
+        const unsigned g = base + b, e = blocks + b;
+        const int slot = g % S;
+        ok = warp_wait(&k_full[slot], g / S & 1, give);
+        if (ok && e >= 2) ok = warp_wait(&pv_done[w][e & 1], (e - 2) >> 1 & 1, give);
+        if (!ok) return;
+        if (elect_one()) {
+          fence_after();
+          const uint64_t db = dk + (uint64_t)(slot * (Lay::block >> 4));
+          const uint32_t d = ts + (e & 1) * kKeys;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          if (i >= tiles) continue;
-          if (pv[i] < qk[i]) {  // weights that may be there
-            const int b = pv[i];
-            const unsigned g = base + b, e = blocks[i] + b;
-            const int slot = g % S;
-            if (__all_sync(kFull, bar_test(&p_full[i][e & 1], e >> 1 & 1) && bar_test(&v_full[slot], g / S & 1))) {
-              if (cleaned < b) {  // once per value block
-                cleaned = b;
-                const int j0 = (c.blk0 + from + b) * kKeys;
-                const int z0 = max(lo - j0, 0), z1 = min(hi - j0, kKeys);  // rows to keep
-                if (z0 > 0 || z1 < kKeys) {
-                  unsigned char* v = sm + Lay::v + slot * Lay::block;
-                  for (int r = lane >> 3; r < kKeys; r += 4)
-                    if (r < z0 || r >= z1)
-#pragma unroll
-                      for (int h = 0; h < DP / 64; h++)
-                        *(uint4*)(v + h * kKvRun + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                  __syncwarp();
-                }
-              }
-              pv[i]++;
-              if (elect_one()) {
-                fence_after();
-                const uint64_t db = sw128_desc(sm + Lay::v + slot * Lay::block, kKvRun, 1024);
-                const uint32_t a = tmem + i * kTile + (e & 1) * kKeys, d = tmem + 2 * kTile + i * kTile;
-#pragma unroll
-                for (int s = 0; s < kKeys / 16; s++)  // 16 keys = 2,048 bytes of V, 8 columns of P a step
-                  mma_ts(d, a + s * 8, db + (uint64_t)(s * 128), kIdPv, b > 0 || s > 0);
-                mma_commit(&pv_done[i][e & 1]);
-                if (tiles == 1 || pv[i ^ 1] > b) mma_commit(&v_empty[slot]);
-              }
-              moved = true;
-            }
-          }
-          if (qk[i] < n && qk[i] < pv[i] + 2) {  // scores: their buffer's earlier weights have been read
-            const int b = qk[i];
-            const unsigned g = base + b, e = blocks[i] + b;
-            const int slot = g % S;
-            bool ready = bar_test(&k_full[slot], g / S & 1);
-            if (b == 0) ready = ready && bar_test(&q_full[i], items[i] & 1);
-            if (e >= 2) ready = ready && bar_test(&pv_done[i][e & 1], (e - 2) >> 1 & 1);
-            if (__all_sync(kFull, ready)) {
-              qk[i]++;
-              if (elect_one()) {
-                fence_after();
-                const uint64_t da = sw128_desc(sm + Lay::q + i * Lay::tile, 16, 1024);
-                const uint64_t db = sw128_desc(sm + Lay::k + slot * Lay::block, 16, 1024);
-                const uint32_t d = tmem + i * kTile + (e & 1) * kKeys;
-#pragma unroll
-                for (int s = 0; s < DP / 16; s++)  // 16 columns = 32 bytes a step
-                  mma_ss(d, da + (uint64_t)((s / 4) * (kQRun >> 4) + (s % 4) * 2),
-                         db + (uint64_t)((s / 4) * (kKvRun >> 4) + (s % 4) * 2), kIdQk, s > 0);
-                mma_commit(&s_full[i][e & 1]);
-                if (tiles == 1 || qk[i ^ 1] > b) mma_commit(&k_empty[slot]);
-              }
-              moved = true;
-            }
-          }
+          for (int s = 0; s < DP / 16; s++)  // 16 columns = 32 bytes a step
+            mma_ss(d, dq + (uint64_t)((s / 4) * (kQRun >> 4) + (s % 4) * 2),
+                   db + (uint64_t)((s / 4) * (kKvRun >> 4) + (s % 4) * 2), kIdQk, s > 0);
+          mma_commit(&s_full[w][e & 1]);
+          mma_commit(&k_empty[slot]);
         }
-        if (pv[0] == n && (tiles == 1 || pv[1] == n)) break;
-        if (moved) {
-          idle = 0;
-        } else if (++idle == 64) {
-          t0 = gtimer();
-        } else if (idle > 64 && (idle & 63) == 0) {
-          const bool late = gtimer() - t0 > kWaitNs;
-          if (late) {
-            *give.abort = 1;
-            atomicCAS(give.err, 0, 1);
-          }
-          if (__any_sync(kFull, late || *give.abort)) {
-            ok = false;
-            break;
-          }
+      };
+      if (!mine) {  // the other tile alone: this one's share of the ring's bookkeeping
+        for (int b = 0; ok && b < n; b++) {
+          const unsigned g = base + b;
+          if (!(ok = warp_wait(&k_full[g % S], g / S & 1, give))) break;
+          if (lane == 0) bar_arrive(&k_empty[g % S]);
+          if (!(ok = warp_wait(&v_full[g % S], g / S & 1, give))) break;
+          if (lane == 0) bar_arrive(&v_empty[g % S]);
         }
-      }
-      for (int i = 0; i < tiles; i++) {
-        items[i]++;
-        blocks[i] += n;
+      } else {
+        ok = warp_wait(&q_full[w], items & 1, give);
+        if (ok) scores(0);
+        if (ok && n > 1) scores(1);
+        for (int b = 0; ok && b < n; b++) {
+          const unsigned g = base + b, e = blocks + b;
+          const int slot = g % S;
+          if (!(ok = warp_wait(&v_full[slot], g / S & 1, give))) break;
+          const int j0 = (c.blk0 + from + b) * kKeys;
+          const int z0 = max(lo - j0, 0), z1 = min(hi - j0, kKeys);  // rows that the item sees
+          if (z0 > 0 || z1 < kKeys) {  // (both tiles' warps write these zeros)
+            unsigned char* v = sm + Lay::v + slot * Lay::block;
+            for (int r = lane >> 3; r < kKeys; r += 4)
+              if (r < z0 || r >= z1)
+#pragma unroll
+                for (int h = 0; h < DP / 64; h++)
+                  *(uint4*)(v + h * kKvRun + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          if (!(ok = warp_wait(&p_full[w][e & 1], e >> 1 & 1, give))) break;
+          if (elect_one()) {
+            fence_after();
+            const uint64_t db = dv + (uint64_t)(slot * (Lay::block >> 4));
+#pragma unroll
+            for (int s = 0; s < kKeys / 16; s++)  // 16 keys = 2,048 bytes of V, 8 columns of P a step
+              mma_ts(to_, ts + (e & 1) * kKeys + s * 8, db + (uint64_t)(s * 128), kIdPv, b > 0 || s > 0);
+            mma_commit(&pv_done[w][e & 1]);
+            mma_commit(&v_empty[slot]);
+          }
+          if (b + 2 < n) scores(b + 2);
+        }
+        items++;
+        blocks += n;
       }
       base += n;
       if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
