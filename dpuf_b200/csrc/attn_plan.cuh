@@ -100,64 +100,96 @@ struct AttnRun {  // this CTA's run of key blocks
   int ctas;         // CTAs that have blocks
 };
 
-// All threads of the CTA call this together.
+// Key blocks of one KV head of each lane's sequence.  A sequence of many tiles is shared by the
+// lanes (a prompt of 2,048 tokens has up to 128, which one thread would walk for microseconds).
 template <int BM, int BN>
-DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nt = blockDim.x;
-  const int per = (p.a.n_seqs + nt - 1) / nt;
-  const int s0 = min(tid * per, p.a.n_seqs), s1 = min(s0 + per, p.a.n_seqs);
-  auto cost = [&](const AttnSeq& q) {
+DPUF_DEV long long attn_costs(const AttnArgs& p, const AttnSeq& q) {
+  const int lane = threadIdx.x & 31, tiles = attn_tiles<BM>(p, q);
+  long long cost = 0;
+  int b0;
+  unsigned many = __ballot_sync(kFull, tiles > 2);
+  if (tiles <= 2)
+    for (int t = 0; t < tiles; t++) cost += attn_tile_blocks<BM, BN>(p, q, t, &b0);
+  for (; many; many &= many - 1) {
+    const int j = __ffs(many) - 1;
+    const AttnSeq o{__shfl_sync(kFull, q.q0, j), __shfl_sync(kFull, q.qn, j), __shfl_sync(kFull, q.kv, j)};
     long long c = 0;
-    int b0;
-    for (int t = 0, n = attn_tiles<BM>(p, q); t < n; t++) c += attn_tile_blocks<BM, BN>(p, q, t, &b0);
-    return c;
-  };
-  long long mine = 0;
-  for (int s = s0; s < s1; s++) mine += cost(attn_seq(p, s)) * p.a.kv.n_kv;
-  long long incl = mine;
+    for (int t = lane, n = attn_tiles<BM>(p, o); t < n; t += 32) c += attn_tile_blocks<BM, BN>(p, o, t, &b0);
+#pragma unroll
+    for (int i = 16; i; i >>= 1) c += __shfl_xor_sync(kFull, c, i);
+    if (lane == j) cost = c;
+  }
+  return cost;
+}
+DPUF_DEV long long attn_scan(long long v) {  // inclusive, over the warp
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(kFull, incl, o);
-    if (lane >= o) incl += v;
+    const long long t = __shfl_up_sync(kFull, v, o);
+    if (lane >= o) v += t;
   }
-  if (lane == 31) sh.warp_sum[warp] = incl;
+  return v;
+}
+
+// All threads of the CTA call this together.  A warp adds up a run of sequences, 32 at a time; the
+// warp in whose run the CTA's first block lies finds it.
+template <int BM, int BN>
+DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  const int per = (p.a.n_seqs + nw - 1) / nw;
+  const int s0 = min(warp * per, p.a.n_seqs), s1 = min(s0 + per, p.a.n_seqs);
+  auto seq_of = [&](int s) { return s + lane < s1 ? attn_seq(p, s + lane) : AttnSeq{0, 0, 0}; };
+  long long mine = 0;
+  for (int s = s0; s < s1; s += 32) mine += attn_costs<BM, BN>(p, seq_of(s));
+#pragma unroll
+  for (int i = 16; i; i >>= 1) mine += __shfl_xor_sync(kFull, mine, i);
+  mine *= p.a.kv.n_kv;
+  if (lane == 0) sh.warp_sum[warp] = mine;
   __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < (nt >> 5); w++) {
-    if (w < warp) before += sh.warp_sum[w];
-    total += sh.warp_sum[w];
-  }
-  incl += before;
+  const long long sums = attn_scan(lane < nw ? sh.warp_sum[lane] : 0);
   AttnRun r;
-  r.total = total;
-  r.ctas = (int)min((long long)ctas, total);
+  r.total = __shfl_sync(kFull, sums, 31);
+  r.ctas = (int)min((long long)ctas, r.total);
   r.n = 0;
   if (cta >= r.ctas) return r;  // the whole CTA
-  const long long b = total * cta / r.ctas, e = total * (cta + 1) / r.ctas;
+  const long long b = r.total * cta / r.ctas, e = r.total * (cta + 1) / r.ctas;
   r.n = (int)(e - b);
-  if (b >= incl - mine && b < incl) {  // one thread
-    long long at = incl - mine;
-    AttnCursor c;
-    for (int s = s0; s < s1; s++) {
-      c.seq = attn_seq(p, s);
-      const long long k = cost(c.seq);
-      if (b < at + k * p.a.kv.n_kv) {
-        c.s = s;
-        c.head = (int)((b - at) / k);
-        at += c.head * k;
-        c.tiles = attn_tiles<BM>(p, c.seq);
-        for (c.tile = 0;; c.tile++) {
-          c.n_blk = attn_tile_blocks<BM, BN>(p, c.seq, c.tile, &c.blk0);
-          if (b < at + c.n_blk) break;
-          at += c.n_blk;
-        }
-        c.begin = at;
-        c.at = (int)(b - at);
-        break;
+  long long at = __shfl_sync(kFull, sums, warp) - mine;
+  if (b >= at && b < at + mine) {  // one warp
+    for (int s = s0;; s += 32) {
+      AttnCursor c;
+      c.seq = seq_of(s);
+      const long long k = attn_costs<BM, BN>(p, c.seq), end = at + attn_scan(k * p.a.kv.n_kv);
+      const unsigned in = __ballot_sync(kFull, b < end);
+      if (!in) {
+        at = __shfl_sync(kFull, end, 31);
+        continue;
       }
-      at += k * p.a.kv.n_kv;
+      const int j = __ffs(in) - 1;
+      const long long cost = __shfl_sync(kFull, k, j);
+      at = __shfl_sync(kFull, end, j) - cost * p.a.kv.n_kv;
+      c.seq = AttnSeq{__shfl_sync(kFull, c.seq.q0, j), __shfl_sync(kFull, c.seq.qn, j), __shfl_sync(kFull, c.seq.kv, j)};
+      c.s = s + j;
+      c.head = (int)((b - at) / cost);
+      at += c.head * cost;
+      c.tiles = attn_tiles<BM>(p, c.seq);
+      for (int t0 = 0;; t0 += 32) {  // 32 tiles at a time
+        c.n_blk = t0 + lane < c.tiles ? attn_tile_blocks<BM, BN>(p, c.seq, t0 + lane, &c.blk0) : 0;
+        const long long tile_end = at + attn_scan(c.n_blk);
+        const unsigned hit = __ballot_sync(kFull, b < tile_end);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            c.tile = t0 + lane;
+            c.begin = tile_end - c.n_blk;
+            c.at = (int)(b - c.begin);
+            sh.start = c;
+          }
+          break;
+        }
+        at = __shfl_sync(kFull, tile_end, 31);
+      }
+      break;
     }
-    sh.start = c;
   }
   __syncthreads();
   r.cur = sh.start;

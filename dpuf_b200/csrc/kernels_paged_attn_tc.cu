@@ -25,6 +25,11 @@
 // PV and the softmax for both) neither unit was busy half of the time.  The price: at N = 64 the
 // QK reads 6 KB of shared memory per 32 tensor cycles, 1.5 times what it delivers.
 //
+//   warp 11           copies the next item's queries while this one's are in use (two buffers).
+//
+// Results leave by way of the queries' shared memory: a row is a thread's, and 32 rows' pieces in
+// one store cost a cycle a row.
+//
 // Every wait is bounded: one that gives up sets the workspace's error word and the CTA's abort
 // flag, all roles stop, copies in flight are waited for (bounded) and TMEM is freed.
 #include <cuda.h>
@@ -40,12 +45,14 @@ namespace {
 constexpr int kTile = 128;            // rows of a tile
 constexpr int kKeys = 64;             // of a block
 constexpr int kItemRows = 2 * kTile;
-constexpr int kLoadWarp = 8, kMmaWarp = 9;  // kMmaWarp + i: tile i
-constexpr int kThreads = 352;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kQueryWarp = 11;  // kMmaWarp + i: tile i
+constexpr int kThreads = 384;
 // The weights carry a factor 2^7, and so does their sum: at most 2^15, which fp16 holds, while the
 // small ones of a long context keep their bits.
 constexpr float kLift = 7.0f;
 constexpr unsigned long long kWaitNs = 2000000000ull;
+
+typedef unsigned long long u64;
 
 DPUF_DEV uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -182,6 +189,28 @@ DPUF_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+DPUF_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two fp32 values at a time, each rounded as alone.
+DPUF_DEV u64 pair(uint32_t a, uint32_t b) {
+  u64 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+  return d;
+}
+DPUF_DEV void split(u64 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+DPUF_DEV u64 fma2(u64 a, u64 b, u64 c) {
+  u64 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+DPUF_DEV u64 add2(u64 a, u64 b) {
+  u64 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 DPUF_DEV uint32_t pack2(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
   return *(const uint32_t*)&h;
@@ -193,11 +222,11 @@ DPUF_DEV uint32_t pack2(float a, float b, __nv_bfloat16) {
 
 template <int DP>
 struct TileLay {  // shared memory, from a 1,024-byte boundary; operands are 64-column runs of [rows][128 bytes]
-  static constexpr int stages = DP == 128 ? 4 : 6;
+  static constexpr int stages = DP == 128 ? 3 : 6;
   static constexpr int tile = kTile * DP * 2;
   static constexpr int block = kKeys * DP * 2;
-  static constexpr int q = 0;                   // [2][tile]
-  static constexpr int k = q + 2 * tile;        // [stages][block]
+  static constexpr int q = 0;                   // [2 items][2][tile]
+  static constexpr int k = q + 4 * tile;        // [stages][block]
   static constexpr int v = k + stages * block;  // [stages][block]
   static constexpr int bytes = v + stages * block + 1024;
 };
@@ -219,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
   constexpr int S = Lay::stages;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S];
-  __shared__ __align__(8) uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2];
   __shared__ AttnShare share;
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_sh, flag_sh[2];
@@ -241,7 +270,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       bar_init(&v_empty[i], 2);
     }
     for (int i = 0; i < 2; i++) {
-      bar_init(&q_full[i], kTile);
+      bar_init(&q_full[i], 32);
+      bar_init(&q_empty[i], 8);
       for (int h = 0; h < 2; h++) {
         bar_init(&s_full[i][h], 1);
         bar_init(&p_full[i][h], kTile);
@@ -315,15 +345,50 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         const unsigned long long t1 = gtimer();
         while (!bar_try(&v_full[i % S], i / S & 1) && gtimer() - t1 < kWaitNs / 100) {}
       }
+  } else if (warp == kQueryWarp) {
+    // ================================================================ queries, an item ahead
+    constexpr int kCh = DP / 8, kStep = 32 / kCh;  // 16-byte chunks of a row, rows of a pass
+    const int ch = lane % kCh;
+    const bool in = ch * 8 < p.a.kv.head_dim;
+    bool ok = true;
+    for (int left = run.n, seg = 0; ok && left > 0; seg++) {
+      left -= min(c.n_blk, c.at + left) - c.at;
+      if (!(ok = warp_wait(&q_empty[seg & 1], (seg >> 1 & 1) ^ 1, give))) break;
+      const int total = c.seq.qn * p.group, r0 = c.tile * kItemRows;
+      const uint32_t dst = su32(sm + Lay::q + (seg & 1) * 2 * Lay::tile);
+      const int rows = total - r0 > kTile ? kItemRows : kTile;
+      const char* const base = (const char*)p.a.q + ch * 16;
+      int rr = r0 + lane / kCh, tok = rr / p.group, g = rr - tok * p.group;
+#pragma unroll 4
+      for (int r = lane / kCh; r < rows; r += kStep) {
+        const bool have = in && rr < total;
+        const int64_t at = have ? ((int64_t)(c.seq.q0 + tok) * p.a.q_stride[0] +
+                                   (int64_t)(c.head * p.group + g) * p.a.q_stride[1]) * 2 : -(int64_t)ch * 16;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         dst + (r >> 7) * Lay::tile + (ch >> 3) * kQRun + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                     "l"(base + at), "r"(have ? 16 : 0)
+                     : "memory");
+        rr += kStep;
+        g += kStep;
+        while (g >= p.group) {
+          g -= p.group;
+          tok++;
+        }
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(su32(&q_full[seg & 1])) : "memory");
+      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight at exit
   } else if (warp >= kMmaWarp) {
     // ================================================================ MMA of tile w
-    constexpr uint32_t kIdQk = idesc_f16<T>(kKeys, 0), kIdPv = idesc_f16<T>(DP, 1);
+    constexpr uint32_t kIdPv = idesc_f16<T>(DP, 1);
+    const uint32_t id_qk = idesc_f16<T>(kKeys, 0) | (p.a.scale < 0.0f ? 1u << 13 : 0u);  // Q negated
     const int w = warp - kMmaWarp;
-    const uint64_t dq = sw128_desc(sm + Lay::q + w * Lay::tile, 16, 1024);
+    const uint64_t dq0 = sw128_desc(sm + Lay::q + w * Lay::tile, 16, 1024);
     const uint64_t dk = sw128_desc(sm + Lay::k, 16, 1024), dv = sw128_desc(sm + Lay::v, kKvRun, 1024);
     const uint32_t ts = tmem + w * kTile, to_ = tmem + 2 * kTile + w * kTile;
     unsigned base = 0;                // blocks of earlier items
-    unsigned items = 0, blocks = 0;   // of this tile so far
+    unsigned seg = 0, blocks = 0;     // items, and blocks of this tile so far
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
       const int from = c.at, to = min(c.n_blk, c.at + left), n = to - from;
@@ -331,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       int lo, hi;
       item_span(p, c.seq, c.tile, &lo, &hi);
       const bool mine = w == 0 || c.seq.qn * p.group - c.tile * kItemRows > kTile;
+      const uint64_t dq = dq0 + (uint64_t)((seg & 1) * (2 * Lay::tile >> 4));
       // scores of block b into its buffer, whose earlier weights have been read
       auto scores = [&](int b) {
         const unsigned g = base + b, e = blocks + b;
@@ -345,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
 #pragma unroll
           for (int s = 0; s < DP / 16; s++)  // 16 columns = 32 bytes a step
             mma_ss(d, dq + (uint64_t)((s / 4) * (kQRun >> 4) + (s % 4) * 2),
-                   db + (uint64_t)((s / 4) * (kKvRun >> 4) + (s % 4) * 2), kIdQk, s > 0);
+                   db + (uint64_t)((s / 4) * (kKvRun >> 4) + (s % 4) * 2), id_qk, s > 0);
           mma_commit(&s_full[w][e & 1]);
           mma_commit(&k_empty[slot]);
         }
@@ -359,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           if (lane == 0) bar_arrive(&v_empty[g % S]);
         }
       } else {
-        ok = warp_wait(&q_full[w], items & 1, give);
+        ok = warp_wait(&q_full[seg & 1], seg >> 1 & 1, give);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the copies are generic writes
         if (ok) scores(0);
         if (ok && n > 1) scores(1);
         for (int b = 0; ok && b < n; b++) {
@@ -390,9 +457,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           }
           if (b + 2 < n) scores(b + 2);
         }
-        items++;
         blocks += n;
       }
+      seg++;
       base += n;
       if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
     }
@@ -403,48 +470,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     const uint32_t tS = tmem + w * kTile + lanes, tO = tmem + 2 * kTile + w * kTile + lanes;
     // not 0, so that a hidden score (-inf) stays one
     const float sl = fmaxf(fabsf(p.a.scale) * 1.44269504088896341f, 1e-37f);
-    const uint32_t flip = p.a.scale < 0.0f ? 0x80008000u : 0u;  // the sign goes with Q
     const int hd = p.a.kv.head_dim;
-    unsigned blocks = 0;
+    unsigned blocks = 0, seg = 0;
     bool ok = true;
     auto wg_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); };
     for (int left = run.n; ok && left > 0;) {
       const int from = c.at, to = min(c.n_blk, c.at + left), n = to - from;
       left -= n;
       const int total = c.seq.qn * p.group, r0 = c.tile * kItemRows + w * kTile;
+      unsigned char* const qs = sm + Lay::q + ((seg & 1) * 2 + w) * Lay::tile;  // free once the last scores are in
+      uint64_t* const q_done = &q_empty[seg & 1];
+      seg++;
       if (w == 1 && r0 >= total) {  // one tile only
+        if (lane == 0) bar_arrive(q_done);
         if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
         continue;
       }
-      // ---- this tile's queries (the earlier item's products are complete: its last scores were)
-      unsigned char* qs = sm + Lay::q + w * Lay::tile;
-      {
-        constexpr int kCh = DP / 8, kStep = kTile / kCh, kBatch = 8;  // 16-byte chunks of a row, rows of a pass
-        const int ch = t % kCh;
-#pragma unroll 1
-        for (int k0 = 0; k0 < kCh; k0 += kBatch) {
-          uint4 x[kBatch];
-#pragma unroll
-          for (int k = 0; k < kBatch; k++) {  // loads of several passes in flight
-            const int rr = r0 + t / kCh + (k0 + k) * kStep;
-            x[k] = make_uint4(0, 0, 0, 0);
-            if (rr < total && ch * 8 < hd)
-              x[k] = __ldg((const uint4*)((const T*)p.a.q + (int64_t)(c.seq.q0 + rr / p.group) * p.a.q_stride[0] +
-                                          (int64_t)(c.head * p.group + rr % p.group) * p.a.q_stride[1] + ch * 8));
-          }
-#pragma unroll
-          for (int k = 0; k < kBatch; k++) {
-            const int r = t / kCh + (k0 + k) * kStep;
-            x[k].x ^= flip; x[k].y ^= flip; x[k].z ^= flip; x[k].w ^= flip;
-            *(uint4*)(qs + (ch >> 3) * kQRun + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[k];
-          }
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(&q_full[w]);
       const int r = r0 + t;
       const bool live = r < total;
-      const int tok = live ? r / p.group : 0, head = c.head * p.group + (live ? r % p.group : 0);
+      const int tok = live ? r / p.group : 0;
       int lo = 0, hi = 0;
       if (live) attn_span(p, c.seq, tok, tok, &lo, &hi);
       float m = -CUDART_INF_F, l = 0.0f;  // m: the maximum that the weights refer to
@@ -464,10 +508,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         }
         float t4[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) t4[i] = __uint_as_float(s[i]);
+        for (int i = 0; i < 4; i++) t4[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
 #pragma unroll
-        for (int i = 4; i < kKeys; i++) t4[i & 3] = fmaxf(t4[i & 3], __uint_as_float(s[i]));
-        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+        for (int i = 8; i < kKeys; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; e++) t4[e] = max3(t4[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
+        const float top = max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]);
         const bool grow = b == 0 || m == -CUDART_INF_F ? top > m : (top - m) * sl > 8.0f;
         if (__any_sync(kFull, grow)) {
           const float m2 = grow ? top : m;
@@ -488,15 +534,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           }
         }
         const float ref = m == -CUDART_INF_F ? 0.0f : __fmaf_rn(m, sl, -kLift);
-        float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const u64 sl2 = pair(__float_as_uint(sl), __float_as_uint(sl));
+        const u64 ref2 = pair(__float_as_uint(-ref), __float_as_uint(-ref));
+        u64 l2[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < kKeys; i += 2) {
-          const float a = ex2(__fmaf_rn(__uint_as_float(s[i]), sl, -ref));
-          const float e = ex2(__fmaf_rn(__uint_as_float(s[i + 1]), sl, -ref));
-          l4[i / 2 & 3] += a + e;
+          float a, e;
+          split(fma2(pair(s[i], s[i + 1]), sl2, ref2), a, e);
+          a = ex2(a);
+          e = ex2(e);
+          l2[i / 2 & 1] = add2(l2[i / 2 & 1], pair(__float_as_uint(a), __float_as_uint(e)));
           s[i / 2] = pack2(a, e, T());
         }
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        float la, lb;
+        split(add2(l2[0], l2[1]), la, lb);
+        l += la + lb;
         tmem_st32(tS + h * kKeys, s);
         tmem_wait_st();
         fence_before();
@@ -543,42 +595,74 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       }
       if (whole || join) {
         const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
-        const size_t at = ((size_t)(c.seq.q0 + tok) * p.a.n_q + head) * hd;
+        // by way of the queries' shared memory, so that a store covers whole rows and not a piece
+        // of 32 of them; a round is DP * 2 bytes of every row
+        auto write = [&](auto wide) {
+          constexpr bool kF32 = decltype(wide)::value;
+          constexpr int kCh = DP / 8, kDims = kF32 ? 4 : 8;  // chunks of a row and round, dims of a chunk
 #pragma unroll
-        for (int i = 0; i < DP / 64; i++) {
-          uint32_t o[64];
-          if (whole) {
-            tmem_ld32(tO + 64 * i, o);
-            tmem_ld32(tO + 64 * i + 32, o + 32);
-            tmem_wait_ld();
-          } else {
-            const int pr = w * kTile + t;
+          for (int i = 0; i < DP / 64; i++) {
+            uint32_t o[64];
+            if (whole) {
+              tmem_ld32(tO + 64 * i, o);
+              tmem_ld32(tO + 64 * i + 32, o + 32);
+              tmem_wait_ld();
+            } else {
+              const int pr = w * kTile + t;
 #pragma unroll
-            for (int e = 0; e < 64; e++) o[e] = 0;
+              for (int e = 0; e < 64; e++) o[e] = 0;
 #pragma unroll 1
-            for (int cc = c0; cc <= c1; cc++) {
-              const size_t slot = 2 * (size_t)cc + (cc == c0);
-              const float x = __ldcg(&parts.ml[slot * kItemRows + pr]).x;
-              const float* src = parts.o + (slot * DP + 64 * i) * kItemRows + pr;
-              float y[64];
+              for (int cc = c0; cc <= c1; cc++) {
+                const size_t slot = 2 * (size_t)cc + (cc == c0);
+                const float x = __ldcg(&parts.ml[slot * kItemRows + pr]).x;
+                const float* src = parts.o + (slot * DP + 64 * i) * kItemRows + pr;
+                float y[64];
 #pragma unroll
-              for (int e = 0; e < 64; e++) y[e] = __ldcg(src + e * kItemRows);
-              const float f = x == -CUDART_INF_F ? 0.0f : ex2(x - m);
+                for (int e = 0; e < 64; e++) y[e] = __ldcg(src + e * kItemRows);
+                const float f = x == -CUDART_INF_F ? 0.0f : ex2(x - m);
 #pragma unroll
-              for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__fmaf_rn(y[e], f, __uint_as_float(o[e])));
+                for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__fmaf_rn(y[e], f, __uint_as_float(o[e])));
+              }
+            }
+#pragma unroll
+            for (int z = 0; z < 64 / kDims; z++) {
+              const int dim = 64 * i + z * kDims, chunk = dim / kDims % kCh;
+              uint4 x;
+              if (kF32) {
+                x.x = __float_as_uint(__uint_as_float(o[z * 4]) * inv);
+                x.y = __float_as_uint(__uint_as_float(o[z * 4 + 1]) * inv);
+                x.z = __float_as_uint(__uint_as_float(o[z * 4 + 2]) * inv);
+                x.w = __float_as_uint(__uint_as_float(o[z * 4 + 3]) * inv);
+              } else {
+                uint32_t h[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  h[e] = pack2(__uint_as_float(o[(z * 8 + 2 * e) & 63]) * inv,
+                               __uint_as_float(o[(z * 8 + 2 * e + 1) & 63]) * inv, T());
+                x = make_uint4(h[0], h[1], h[2], h[3]);
+              }
+              *(uint4*)(qs + t * (DP * 2) + ((chunk ^ (t & 7)) << 4)) = x;
+              if (chunk == kCh - 1) {  // the round is full
+                wg_sync();
+                const int ch = t % kCh, d0 = dim / (kCh * kDims) * (kCh * kDims) + ch * kDims;
+                if (d0 < hd)
+#pragma unroll 4
+                  for (int rr = t / kCh; rr < kTile && r0 + rr < total; rr += kTile / kCh) {
+                    const int tk = (r0 + rr) / p.group, hh = c.head * p.group + (r0 + rr) - tk * p.group;
+                    const size_t to_at = ((size_t)(c.seq.q0 + tk) * p.a.n_q + hh) * hd + d0;
+                    *(uint4*)((char*)p.a.out + to_at * (kF32 ? 4 : 2)) =
+                        *(const uint4*)(qs + rr * (DP * 2) + ((ch ^ (rr & 7)) << 4));
+                  }
+                wg_sync();
+              }
             }
           }
-          if (live)
-#pragma unroll
-            for (int g = 0; g < 8; g++)
-              if (64 * i + 8 * g < hd) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = __uint_as_float(o[8 * g + e]) * inv;
-                store8_as(p.a.out, at + 64 * i + 8 * g, p.a.out_dtype, x);
-              }
-        }
+        };
+        if (p.a.out_dtype == DPUF_TYPE_F32) write(std::true_type());
+        else write(std::false_type());
       }
+      __syncwarp();
+      if (lane == 0) bar_arrive(q_done);
       fence_before();  // O is read: the next item's products may overwrite it once its P arrives
       if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
     }
