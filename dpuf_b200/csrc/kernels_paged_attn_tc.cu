@@ -235,6 +235,8 @@ constexpr int kQRun = kTile * 128, kKvRun = kKeys * 128;  // bytes of a 64-colum
 struct TileArgs {
   AttnArgs p;
   CUtensorMap k_map, v_map;  // (dim, row, head, page), boxes of 64 x min(page_size, 64)
+  CUtensorMap q_map;         // (dim, head, token), boxes of 64 x group x 128 / group: a tile's rows
+  int q_boxes;               // whether q_map is usable: the group divides 128
 };
 
 // Positions that an item's rows [r0, r0 + rows) see between them.
@@ -357,8 +359,29 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       const int total = c.seq.qn * p.group, r0 = c.tile * kItemRows;
       const uint32_t dst = su32(sm + Lay::q + (seg & 1) * 2 * Lay::tile);
       const int rows = total - r0 > kTile ? kItemRows : kTile;
+      if (args.q_boxes) {  // rows beyond the sequence are the next one's or zeros: nobody reads their results
+        if (lane == 0) {
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(&q_full[seg & 1])),
+                       "r"(rows / kTile * Lay::tile)
+                       : "memory");
+          for (int i = 0; i < rows / kTile; i++)
+#pragma unroll
+            for (int h = 0; h < DP / 64; h++)
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+                  "%3, %4}], [%5];" ::"r"(dst + i * Lay::tile + h * kQRun),
+                  "l"(&args.q_map), "r"(h * 64), "r"(c.head * p.group), "r"(c.seq.q0 + (r0 + i * kTile) / p.group),
+                  "r"(su32(&q_full[seg & 1]))
+                  : "memory");
+        } else {
+          bar_arrive(&q_full[seg & 1]);
+        }
+        if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+        continue;
+      }
       const char* const base = (const char*)p.a.q + ch * 16;
       int rr = r0 + lane / kCh, tok = rr / p.group, g = rr - tok * p.group;
+      const int step_t = kStep / p.group, step_g = kStep - step_t * p.group;
 #pragma unroll 4
       for (int r = lane / kCh; r < rows; r += kStep) {
         const bool have = in && rr < total;
@@ -369,8 +392,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
                      "l"(base + at), "r"(have ? 16 : 0)
                      : "memory");
         rr += kStep;
-        g += kStep;
-        while (g >= p.group) {
+        tok += step_t;
+        g += step_g;
+        if (g >= p.group) {
           g -= p.group;
           tok++;
         }
@@ -645,14 +669,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
               if (chunk == kCh - 1) {  // the round is full
                 wg_sync();
                 const int ch = t % kCh, d0 = dim / (kCh * kDims) * (kCh * kDims) + ch * kDims;
-                if (d0 < hd)
+                if (d0 < hd) {
+                  // token and head of the first row, and their steps
+                  int tk = (r0 + t / kCh) / p.group, hh = r0 + t / kCh - tk * p.group;
+                  const int step_t = kTile / kCh / p.group, step_h = kTile / kCh - step_t * p.group;
 #pragma unroll 4
-                  for (int rr = t / kCh; rr < kTile && r0 + rr < total; rr += kTile / kCh) {
-                    const int tk = (r0 + rr) / p.group, hh = c.head * p.group + (r0 + rr) - tk * p.group;
-                    const size_t to_at = ((size_t)(c.seq.q0 + tk) * p.a.n_q + hh) * hd + d0;
-                    *(uint4*)((char*)p.a.out + to_at * (kF32 ? 4 : 2)) =
-                        *(const uint4*)(qs + rr * (DP * 2) + ((ch ^ (rr & 7)) << 4));
+                  for (int rr = t / kCh; rr < kTile; rr += kTile / kCh) {
+                    const size_t to_at = ((size_t)(c.seq.q0 + tk) * p.a.n_q + c.head * p.group + hh) * hd + d0;
+                    if (r0 + rr < total)
+                      *(uint4*)((char*)p.a.out + to_at * (kF32 ? 4 : 2)) =
+                          *(const uint4*)(qs + rr * (DP * 2) + ((ch ^ (rr & 7)) << 4));
+                    tk += step_t;
+                    hh += step_h;
+                    if (hh >= p.group) {
+                      hh -= p.group;
+                      tk++;
+                    }
                   }
+                }
                 wg_sync();
               }
             }
@@ -689,14 +723,14 @@ EncodeFn encoder() {
   return fn;
 }
 
-bool encode(CUtensorMap* map, const DpufPagedKv& kv, void* base) {
-  const cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_kv,
-                              (cuuint64_t)kv.n_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)kv.row_stride * 2, (cuuint64_t)kv.head_stride * 2,
-                                 (cuuint64_t)kv.page_stride * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(kv.page_size, kKeys), 1, 1}, one[4] = {1, 1, 1, 1};
-  return encoder()(map, kv.dtype == DPUF_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                   4, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+// `strides` of dimensions 1.. in elements of 2 bytes.
+bool encode(CUtensorMap* map, int dtype, void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box) {
+  cuuint64_t bytes[3];
+  for (int i = 0; i + 1 < rank; i++) bytes[i] = strides[i] * 2;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return encoder()(map, dtype == DPUF_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                   rank, base, dims, bytes, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -716,9 +750,19 @@ cudaError_t launch_paged_attention_tc(const AttnArgs& p, cudaStream_t s) {
   if (!encoder()) return cudaErrorNotSupported;
   TileArgs a;
   a.p = p;
-  if (!encode(&a.k_map, p.a.kv, p.a.kv.k) || !encode(&a.v_map, p.a.kv, p.a.kv.v)) return cudaErrorInvalidValue;
-  const bool small = p.a.kv.head_dim <= 64;
-  if (p.a.kv.dtype == DPUF_TYPE_F16) return small ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+  const DpufPagedKv& kv = p.a.kv;
+  const cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_kv,
+                              (cuuint64_t)kv.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)kv.row_stride, (cuuint64_t)kv.head_stride, (cuuint64_t)kv.page_stride};
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(kv.page_size, kKeys), 1, 1};
+  if (!encode(&a.k_map, kv.dtype, kv.k, 4, dims, strides, box) || !encode(&a.v_map, kv.dtype, kv.v, 4, dims, strides, box))
+    return cudaErrorInvalidValue;
+  const cuuint64_t q_dims[3] = {(cuuint64_t)kv.head_dim, (cuuint64_t)p.a.n_q, (cuuint64_t)p.a.n_tokens};
+  const cuuint64_t q_strides[2] = {(cuuint64_t)p.a.q_stride[1], (cuuint64_t)p.a.q_stride[0]};
+  const cuuint32_t q_box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(kTile / p.group)};
+  a.q_boxes = kTile % p.group == 0 && encode(&a.q_map, kv.dtype, (void*)p.a.q, 3, q_dims, q_strides, q_box);
+  const bool small = kv.head_dim <= 64;
+  if (kv.dtype == DPUF_TYPE_F16) return small ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
   return small ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
 }
 
