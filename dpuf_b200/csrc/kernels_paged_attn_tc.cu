@@ -235,8 +235,8 @@ constexpr int kQRun = kTile * 128, kKvRun = kKeys * 128;  // bytes of a 64-colum
 struct TileArgs {
   AttnArgs p;
   CUtensorMap k_map, v_map;  // (dim, row, head, page), boxes of 64 x min(page_size, 64)
-  CUtensorMap q_map;         // (dim, head, token), boxes of 64 x group x 128 / group: a tile's rows
-  int q_boxes;               // whether q_map is usable: the group divides 128
+  CUtensorMap q_map, o_map;  // (dim, head, token), boxes of 64 x group x 128 / group: a tile's rows
+  int q_boxes, o_boxes;      // whether they are usable: the group divides 128, out has q's type
 };
 
 // Positions that an item's rows [r0, r0 + rows) see between them.
@@ -496,6 +496,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     const float sl = fmaxf(fabsf(p.a.scale) * 1.44269504088896341f, 1e-37f);
     const int hd = p.a.kv.head_dim;
     unsigned blocks = 0, seg = 0;
+    uint64_t* pending = nullptr;  // to arrive on once the TMA store has read the buffer (thread 0)
+    auto stored = [&]() {
+      if (pending) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        bar_arrive(pending);
+        pending = nullptr;
+      }
+    };
     bool ok = true;
     auto wg_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); };
     for (int left = run.n; ok && left > 0;) {
@@ -577,6 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         tmem_wait_st();
         fence_before();
         bar_arrive(&p_full[w][h]);
+        stored();  // the item before's, long read by now
       }
       if (!ok || !(ok = warp_wait(&pv_done[w][(blocks - 1) & 1], (blocks - 1) >> 1 & 1, give))) break;
       fence_after();
@@ -620,7 +629,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       if (whole || join) {
         const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
         // by way of the queries' shared memory, so that a store covers whole rows and not a piece
-        // of 32 of them; a round is DP * 2 bytes of every row
+        // of 32 of them; a round is DP * 2 bytes of every row.  A full tile in q's type leaves by
+        // TMA, which the next item's first block does not wait for.
+        const bool boxes = args.o_boxes && r0 + kTile <= total;
+        if (boxes && t == 0) pending = q_done;
         auto write = [&](auto wide) {
           constexpr bool kF32 = decltype(wide)::value;
           constexpr int kCh = DP / 8, kDims = kF32 ? 4 : 8;  // chunks of a row and round, dims of a chunk
@@ -665,8 +677,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
                                __uint_as_float(o[(z * 8 + 2 * e + 1) & 63]) * inv, T());
                 x = make_uint4(h[0], h[1], h[2], h[3]);
               }
-              *(uint4*)(qs + t * (DP * 2) + ((chunk ^ (t & 7)) << 4)) = x;
+              *(uint4*)(qs + (chunk >> 3) * kQRun + t * 128 + (((chunk & 7) ^ (t & 7)) << 4)) = x;
               if (chunk == kCh - 1) {  // the round is full
+                if (!kF32 && boxes) {
+                  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                  wg_sync();
+                  if (t == 0) {
+#pragma unroll
+                    for (int h = 0; h < DP / 64; h++)
+                      asm volatile(
+                          "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                              &args.o_map),
+                          "r"(h * 64), "r"(c.head * p.group), "r"(c.seq.q0 + r0 / p.group), "r"(su32(qs + h * kQRun))
+                          : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                  }
+                  continue;
+                }
                 wg_sync();
                 const int ch = t % kCh, d0 = dim / (kCh * kDims) * (kCh * kDims) + ch * kDims;
                 if (d0 < hd) {
@@ -678,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
                     const size_t to_at = ((size_t)(c.seq.q0 + tk) * p.a.n_q + c.head * p.group + hh) * hd + d0;
                     if (r0 + rr < total)
                       *(uint4*)((char*)p.a.out + to_at * (kF32 ? 4 : 2)) =
-                          *(const uint4*)(qs + rr * (DP * 2) + ((ch ^ (rr & 7)) << 4));
+                          *(const uint4*)(qs + (ch >> 3) * kQRun + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
                     tk += step_t;
                     hh += step_h;
                     if (hh >= p.group) {
@@ -696,10 +723,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         else write(std::false_type());
       }
       __syncwarp();
-      if (lane == 0) bar_arrive(q_done);
+      if (lane == 0 && !pending) bar_arrive(q_done);
       fence_before();  // O is read: the next item's products may overwrite it once its P arrives
       if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
     }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // nothing in flight at exit
   }
   fence_before();
   __syncthreads();
@@ -761,6 +789,8 @@ cudaError_t launch_paged_attention_tc(const AttnArgs& p, cudaStream_t s) {
   const cuuint64_t q_strides[2] = {(cuuint64_t)p.a.q_stride[1], (cuuint64_t)p.a.q_stride[0]};
   const cuuint32_t q_box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(kTile / p.group)};
   a.q_boxes = kTile % p.group == 0 && encode(&a.q_map, kv.dtype, (void*)p.a.q, 3, q_dims, q_strides, q_box);
+  const cuuint64_t o_strides[2] = {(cuuint64_t)kv.head_dim, (cuuint64_t)p.a.n_q * kv.head_dim};
+  a.o_boxes = a.q_boxes && p.a.out_dtype == p.a.dtype && encode(&a.o_map, kv.dtype, p.a.out, 3, q_dims, o_strides, q_box);
   const bool small = kv.head_dim <= 64;
   if (kv.dtype == DPUF_TYPE_F16) return small ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
   return small ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
