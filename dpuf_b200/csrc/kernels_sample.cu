@@ -4,20 +4,21 @@
 // With m the row's maximum, an entry's weight is w = exp((l - m) / T) in fp32, taken into sums
 // as the integer f = round(w 2^43): sums of integers do not depend on their order, so neither do
 // the thresholds and the id (an entry below 2^-44 of the maximum's weight has f = 0 and is never
-// kept).  All three filters keep a prefix of the order (logit down, index up), i.e. all entries
+// kept; rounding down instead would lose half a unit an entry, and 10^5 entries' worth moves ids).  All three filters keep a prefix of the order (logit down, index up), i.e. all entries
 // above a threshold value and the first few, by index, of those equal to it.  No sort of the row:
 //
 //  1. the row's slices go to the cluster's shared memory, once; the maximum.
-//  2. a histogram of counts over 1,024 equal steps of (m - l) / T, summed over the cluster.  The
+//  2. a histogram of counts over 1,024 equal steps of (m - l) / T down to the smallest entry, or
+//     to where weights end, summed over the cluster.  The
 //     step in which top-k ends follows exactly, for top-p a step by which it has ended for sure
 //     (a step's weight is between its count times its ends' weights), for min-p the same.
-//  3. the entries down to that step are compacted, in index order, and moved to one CTA of the
-//     cluster (the others are then done): mostly a few dozen.
-//  4. up to 512 of them it sorts, and applies the filters on running sums.  Of more, the thresholds
-//     are searched by histograms of counts and weights over ranges of the value's bits (made
-//     monotone), each range the bin of the one before, until it is one value.  Where they are too
-//     many to move (a nucleus of much of the vocabulary) the cluster does the same together, each
-//     CTA adding up one segment of the bins.
+//  3. the entries down to that step are handed to one CTA of the cluster (the others are then
+//     done): mostly a few dozen.
+//  4. up to 256 of them, a thread each, it ranks by comparing all with all, which gives each one's
+//     running weight too.  Of more, the thresholds are searched by histograms of counts and weights
+//     over ranges of the value's bits (made monotone), each range the bin of the one before, until
+//     it is one value.  Where they are too many to hand over (a nucleus of much of the vocabulary)
+//     the cluster does the same together, each CTA adding up one segment of the bins.
 //  5. the running weight in index order passes u times the kept weight at the id.
 //
 // Bound by latency for few rows (the cluster's barriers and the block's), by the passes over the
@@ -39,8 +40,8 @@ constexpr int kSampThreads = 512;
 constexpr int kSampWarps = kSampThreads / 32;
 constexpr int kBins = 1024;
 constexpr int kMaxCluster = 16;
-constexpr int kListCap = 1024;            // entries that one CTA hands over
-constexpr int kSortCap = kSampThreads;    // entries that one CTA sorts
+constexpr int kListCap = 3072;            // entries that one CTA hands over
+constexpr int kFewCap = 256;              // entries that are ranked by comparison
 constexpr float kFix = 8796093022208.0f;  // 2^43
 constexpr float kReach = 30.6f;           // > 44 ln 2: beyond it f is 0
 
@@ -84,25 +85,32 @@ struct Found {  // the bin in which a running sum reaches its target, and the su
 
 struct SampleShared {
   uint32_t count[kBins];
-  union {
+  union {  // one after the other
+    struct {  // what a CTA hands over, in index order
+      float list_v[kListCap];
+      int list_i[kListCap];
+    };
     struct {
       uint32_t m0[kBins], m1[kBins], m2[kBins];  // weights in three parts of 15 bits
+      uint32_t bin_count[kBins];                 // this CTA's segment of the bins, summed over the CTAs
+      u64 bin_mass[kBins];
     };
-    u64 sorted[kSortCap];
   };
-  uint32_t bin_count[kBins];  // this CTA's segment of the bins, summed over the CTAs
-  u64 bin_mass[kBins];
-  float list_v[kListCap];
-  int list_i[kListCap];
+  float few_v[kFewCap];  // in rank 0: the entries in no order,
+  int few_i[kFewCap];    // ranked ones' weights
+  u64 few_f[kFewCap], few_x[kFewCap];
+  unsigned few_n;
+  uint32_t first;  // where this CTA's entries go
   uint32_t seg_count;
   u64 seg_mass;
   u64 best;  // maximum's key and lowest index
+  float low;  // minimum
   u64 exchange[4];
   u64 warp_sum[kSampWarps];
-  double warp_lo[kSampWarps], warp_hi[kSampWarps];
+  float warp_lo[kSampWarps], warp_hi[kSampWarps];
   Found found;
   int step_k, step_p;
-  double hi_k;
+  float hi_k, hi_m;
 };
 
 DPUF_DEV u64 warp_inclusive(u64 v) {
@@ -110,6 +118,15 @@ DPUF_DEV u64 warp_inclusive(u64 v) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const u64 t = __shfl_up_sync(kFull, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+DPUF_DEV uint32_t warp_inclusive32(uint32_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t t = __shfl_up_sync(kFull, v, o);
     if (lane >= o) v += t;
   }
   return v;
@@ -138,7 +155,7 @@ DPUF_DEV u64 block_sum(u64 v, u64* warp_sum) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char dyn[];
   SampleShared& sh = *(SampleShared*)dyn;
   T* cache = (T*)(dyn + ((sizeof(SampleShared) + 15) & ~(size_t)15));
@@ -169,11 +186,13 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   // ---- 1. the slice, and the row's maximum (lowest index)
   float top_v = -CUDART_INF_F;
   int top_i = -1;
+  float low_v = CUDART_INF_F;
   auto see = [&](float v, int i) {
     if (v > top_v) {
       top_v = v;
       top_i = i;
     }
+    low_v = fminf(low_v, v);
   };
   const bool vectors = ((uintptr_t)src & 15) == 0;
   constexpr int kVec = 16 / sizeof(T);
@@ -196,17 +215,28 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   u64 best = top_i < 0 ? 0 : ((u64)Key<T>::of(top_v) << 32) | (uint32_t)~(uint32_t)(base + top_i);
 #pragma unroll
   for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
-  if (lane == 0) sh.warp_sum[tid >> 5] = best;
+  low_v = -warp_max(-low_v);
+  if (lane == 0) {
+    sh.warp_sum[tid >> 5] = best;
+    sh.warp_lo[tid >> 5] = low_v;
+  }
   for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = 0;
+  if (tid == 0) sh.few_n = 0;
   __syncthreads();
   if (tid < 32) {
     best = lane < kSampWarps ? sh.warp_sum[lane] : 0;
+    low_v = lane < kSampWarps ? sh.warp_lo[lane] : CUDART_INF_F;
 #pragma unroll
     for (int o = kSampWarps / 2; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
-    if (lane == 0) sh.best = best;
+    low_v = -warp_max(-low_v);
+    if (lane == 0) {
+      sh.best = best;
+      sh.low = low_v;
+    }
   }
   cl.sync();
   best = lane < R ? of(lane)->best : 0;
+  low_v = -warp_max(lane < R ? -of(lane)->low : -CUDART_INF_F);
 #pragma unroll
   for (int o = kMaxCluster / 2; o; o >>= 1) best = max(best, __shfl_xor_sync(kFull, best, o));
   best = __shfl_sync(kFull, best, 0);
@@ -231,11 +261,19 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     const float w = v == m ? 1.0f : expf((v - m) * inv_t);
     return w > 0.0f ? w : 0.0f;  // NaN has none
   };
-  auto fixed = [&](float w) { return (u64)__float2ull_rn(w * kFix); };
-  const float per_step = (float)kBins / kReach;  // steps per unit of (m - l) / T
-  auto step_of = [&](float v) {                  // -1: beyond the reach, or NaN
+  // round(w 2^43) of w in [0, 1]: the 24-bit significand, shifted (half up)
+  auto fixed = [&](float w) -> u64 {
+    const uint32_t b = __float_as_uint(w);
+    const int n = 146 - (int)(b >> 23);
+    return n > 63 ? 0 : (((u64)((b & 0x7FFFFFu) | 0x800000u) << 39) + (1ull << (n - 1))) >> n;
+  };
+  // steps per unit of (m - l) / T; a little more than the row's span, so that its smallest entry is inside
+  const float span = (m - low_v) * inv_t * 1.0001f + 1e-6f;
+  const float reach = span < kReach ? span : kReach;  // (kReach for an infinite or undefined span)
+  const float per_step = (float)kBins / reach;
+  auto step_of = [&](float v) {  // -1: beyond the reach, or NaN
     const float z = v == m ? 0.0f : (m - v) * inv_t;
-    return z < kReach ? min((int)(z * per_step), kBins - 1) : -1;
+    return z < reach ? min((int)(z * per_step), kBins - 1) : -1;
   };
   // every entry of the slice, in no order: 16 bytes at a time
   auto each = [&](auto f) {
@@ -259,22 +297,22 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
   u64 mass = 0;                     // weight of what top-k keeps, where by_p
   int last_step = kBins;            // kBins: the whole slice stays the domain
   if (limit_k || limit_p) {
-    u64 mine = 0;
-    const bool want_mass = limit_p && !limit_k;
-    each([&](float v) {
-      const int b = step_of(v);
-      if (b >= 0) {
-        atomicAdd(&sh.count[b], 1u);
-        if (want_mass) mine += fixed(weight(v));
-      }
-    });
-    if (want_mass) {
+    auto whole_mass = [&]() {
+      u64 mine = 0;
+      each([&](float v) { mine += fixed(weight(v)); });
       mine = block_sum(mine, sh.warp_sum);
       if (tid == 0) sh.exchange[0] = mine;
-    }
+    };
+    each([&](float v) {
+      const int b = step_of(v);
+      if (b >= 0) atomicAdd(&sh.count[b], 1u);
+    });
+    const bool mass_now = limit_p && !limit_k && !(min_p > 0.0f);  // else it may not be needed
+    if (mass_now) whole_mass();
     cl.sync();
-    if (want_mass) mass = over_cluster(0);
-    // bins 2 tid and 2 tid + 1: counts, and bounds of their weights
+    if (mass_now) mass = over_cluster(0);
+    // bins 2 tid and 2 tid + 1: counts, and bounds of their weights (wide enough for the rounding
+    // of the sums)
     uint32_t c[2] = {0, 0};
 #pragma unroll 8
     for (int r = 0; r < R; r++) {
@@ -282,71 +320,74 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
       c[0] += x.x;
       c[1] += x.y;
     }
-    double lo[2], hi[2];
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int b = 2 * tid + e;
-      hi[e] = c[e] * (double)(b == 0 ? 1.0f : expf(-(float)b / per_step) * 1.0001f);
-      lo[e] = b == kBins - 1 ? 0.0 : c[e] * (double)(expf(-(float)(b + 1) / per_step) * 0.9999f);
-    }
-    u64 cc = block_inclusive((u64)c[0] + c[1], sh.warp_sum);
-    double cl_ = lo[0] + lo[1], ch = hi[0] + hi[1];
+    const float w0 = expf(-(float)(2 * tid) / per_step), w1 = expf(-(float)(2 * tid + 1) / per_step),
+                w2 = tid == kSampThreads - 1 ? 0.0f : expf(-(float)(2 * tid + 2) / per_step);
+    const float hi[2] = {c[0] * w0 * 1.001f, c[1] * w1 * 1.001f}, lo[2] = {c[0] * w1 * 0.999f, c[1] * w2 * 0.999f};
+    uint32_t cc = c[0] + c[1];
+    float sl = lo[0] + lo[1], sh_ = hi[0] + hi[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_up_sync(kFull, cl_, o), y = __shfl_up_sync(kFull, ch, o);
+      const uint32_t z = __shfl_up_sync(kFull, cc, o);
+      const float x = __shfl_up_sync(kFull, sl, o), y = __shfl_up_sync(kFull, sh_, o);
       if (lane >= o) {
-        cl_ += x;
-        ch += y;
+        cc += z;
+        sl += x;
+        sh_ += y;
       }
     }
     if (lane == 31) {
-      sh.warp_lo[tid >> 5] = cl_;
-      sh.warp_hi[tid >> 5] = ch;
+      sh.warp_sum[tid >> 5] = cc;
+      sh.warp_lo[tid >> 5] = sl;
+      sh.warp_hi[tid >> 5] = sh_;
     }
     if (tid == 0) sh.step_k = sh.step_p = kBins;
     __syncthreads();
-    for (int w = 0; w < (tid >> 5); w++) {
-      cl_ += sh.warp_lo[w];
-      ch += sh.warp_hi[w];
+    float all_lo = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSampWarps; w++) {
+      if (w < (tid >> 5)) {
+        cc += (uint32_t)sh.warp_sum[w];
+        sl += sh.warp_lo[w];
+        sh_ += sh.warp_hi[w];
+      }
+      all_lo += sh.warp_lo[w];
     }
     // running sums at the ends of bins 2 tid and 2 tid + 1
-    const u64 run[2] = {cc - c[1], cc};
-    const double run_lo[2] = {cl_ - lo[1], cl_}, run_hi[2] = {ch - hi[1], ch};
-    if (limit_k)
+    const uint32_t run[2] = {cc - c[1], cc};
+    const float run_lo[2] = {sl - lo[1], sl}, run_hi[2] = {sh_ - hi[1], sh_};
+    const int step_m = min_p > 0.0f ? min((int)(-logf(min_p) * per_step * 1.0001f) + 1, kBins - 1) : kBins - 1;
 #pragma unroll
-      for (int e = 0; e < 2; e++)
-        if (run[e] > (u64)k && run[e] - c[e] <= (u64)k) {  // strictly more than k up to here
-          sh.step_k = 2 * tid + e;
-          sh.hi_k = run_hi[e];
-        }
+    for (int e = 0; e < 2; e++) {
+      if (limit_k && run[e] > (uint32_t)k && run[e] - c[e] <= (uint32_t)k) {  // strictly more than k up to here
+        sh.step_k = 2 * tid + e;
+        sh.hi_k = run_hi[e];
+      }
+      if (2 * tid + e == step_m) sh.hi_m = run_hi[e];
+    }
     __syncthreads();
     by_k = limit_k && sh.step_k < kBins;
-    by_p = limit_p;
-    if (by_p && limit_k && !by_k) {  // the weight of everything is needed after all
-      u64 mine2 = 0;
-      each([&](float v) { mine2 += fixed(weight(v)); });
-      mine2 = block_sum(mine2, sh.warp_sum);
-      if (tid == 0) sh.exchange[0] = mine2;
+    // min-p may end the prefix before top-p for sure
+    by_p = limit_p && (by_k || min_p <= 0.0f || sh.hi_m >= top_p * all_lo * 0.999f);
+    if (by_p && !by_k && !mass_now) {
+      whole_mass();
       cl.sync();
       mass = over_cluster(0);
     }
     if (by_p) {
       // at most the upper bound of top-k's weight where it is not known yet
-      const double target = (double)top_p * (by_k ? sh.hi_k : (double)mass / (double)kFix) * 1.0001;
+      const float target = top_p * (by_k ? sh.hi_k : (float)((double)mass / (double)kFix)) * 1.001f;
 #pragma unroll
       for (int e = 0; e < 2; e++)
-        if (run_lo[e] >= target && run_lo[e] - lo[e] < target) atomicMin(&sh.step_p, 2 * tid + e);
+        if (run_lo[e] >= target && (2 * tid + e == 0 || run_lo[e] - lo[e] < target)) atomicMin(&sh.step_p, 2 * tid + e);
       __syncthreads();
     }
     // top-p after a top-k that ends the prefix needs all that top-k keeps for its weight
     last_step = by_k ? sh.step_k : sh.step_p;
-    if (min_p > 0.0f && !(by_k && by_p)) last_step = min(last_step, (int)(-logf(min_p) * per_step * 1.0001f) + 1);
+    if (min_p > 0.0f && !(by_k && by_p)) last_step = min(last_step, step_m);
   }
 
-  // ---- 3. the entries down to that step, in index order (a thread's run of the slice is
-  // contiguous and of odd length: no bank conflicts), moved to rank 0
-  const int per = ((n + kSampThreads - 1) / kSampThreads) | 1;
-  const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  // ---- 3. the entries down to that step to rank 0: at once while they are few, else once its
+  // slice is free.  In index order: a warp has a run of the slice, a lane 16 bytes of each step.
   float cut = -CUDART_INF_F;
   bool local = false;  // rank 0 goes on alone, over what it has been given
   int have = 0;
@@ -356,26 +397,82 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     const float low = m - (float)(last_step + 1) / per_step * temp;
     cut = fminf(low - 1e-5f * (fabsf(m) + fabsf(low)) - 1e-30f, m);  // at or below every entry wanted
     if (!(cut <= m)) cut = -CUDART_INF_F;                             // the step's end is not finite
+    constexpr int kStep = 32 * kVec;
+    const int steps = (n + kStep - 1) / kStep, warp = tid >> 5;
+    const int s0 = steps * warp / kSampWarps, s1 = steps * (warp + 1) / kSampWarps;
+    auto lane_values = [&](int s, float (&v)[kVec]) {  // NaN beyond the slice
+      const int i = s * kStep + lane * kVec;
+      if (i + kVec <= min(n, a.cached)) {
+        const uint4 x = *(const uint4*)(cache + i);
+        const T* e = (const T*)&x;
+#pragma unroll
+        for (int j = 0; j < kVec; j++) v[j] = to_f32(e[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; j++) v[j] = i + j < n ? at(i + j) : CUDART_NAN_F;
+      }
+    };
     uint32_t mine = 0;
-    for (int i = i0; i < i1; i++) mine += at(i) >= cut;
-    const uint32_t incl = (uint32_t)block_inclusive(mine, sh.warp_sum);
-    if (incl <= kListCap && mine) {
-      uint32_t o = incl - mine;
-      for (int i = i0; i < i1; i++) {
-        const float v = at(i);
-        if (v >= cut) {
-          sh.list_v[o] = v;
-          sh.list_i[o++] = base + i;
-        }
+    for (int s = s0; s < s1; s++) {
+      float v[kVec];
+      lane_values(s, v);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) mine += v[j] >= cut;
+    }
+    const uint32_t of_warp = __reduce_add_sync(kFull, mine);
+    if (lane == 0) sh.warp_sum[warp] = of_warp;
+    __syncthreads();
+    uint32_t o = 0, all = 0;  // where the warp's entries begin, the CTA's entries
+#pragma unroll
+    for (int w = 0; w < kSampWarps; w++) {
+      if (w < warp) o += (uint32_t)sh.warp_sum[w];
+      all += (uint32_t)sh.warp_sum[w];
+    }
+    if (tid == 0) {
+      sh.exchange[1] = all <= kListCap ? all : 1u << 30;
+      sh.first = all == 0 ? 0 : atomicAdd(&of(0)->few_n, all);
+    }
+    __syncthreads();
+    SampleShared* const to = of(0);
+    if (of_warp && all <= kListCap) {
+      const uint32_t first = sh.first;
+      const bool few = first < kFewCap && all <= kFewCap;
+      for (int s = s0; s < s1; s++) {
+        float v[kVec];
+        lane_values(s, v);
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < kVec; j++) in |= (uint32_t)(v[j] >= cut) << j;
+        if (!__any_sync(kFull, in != 0)) continue;
+        const uint32_t incl = (uint32_t)warp_inclusive32(__popc(in));
+        uint32_t at_ = o + incl - __popc(in);
+#pragma unroll
+        for (int j = 0; j < kVec; j++)
+          if (in >> j & 1) {
+            const int id = base + s * kStep + lane * kVec + j;
+            if (few && first + at_ < kFewCap) {
+              to->few_v[first + at_] = v[j];
+              to->few_i[first + at_] = id;
+            }
+            sh.list_v[at_] = v[j];
+            sh.list_i[at_++] = id;
+          }
+        o += __shfl_sync(kFull, incl, 31);
       }
     }
-    if (tid == kSampThreads - 1) sh.exchange[1] = incl <= kListCap ? incl : 1u << 30;
     cl.sync();  // rank 0's slice is not needed any more if the lists fit
     const u64 entries = over_cluster(1);
-    if (entries <= (u64)a.given) {
+    if (entries <= kFewCap) {
+      have = (int)entries;
+      local = true;
+      cl.barrier_arrive();  // this CTA has read the others' counts; they wait for that before they leave
+      if (rank != 0) {
+        cl.barrier_wait();
+        return;
+      }
+    } else if (entries <= (u64)a.given) {
       local = true;
       have = (int)entries;
-      SampleShared* const to = of(0);
       T* const tv = (T*)((unsigned char*)to + ((unsigned char*)given_v - dyn));
       int* const ti = (int*)((unsigned char*)to + ((unsigned char*)given_i - dyn));
       const int first = (int)below_rank(1), mine_n = (int)sh.exchange[1];
@@ -390,51 +487,53 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
     cl.sync();  // the counts are read: the histograms below may overwrite them
   }
 
-  if (local && have <= kSortCap) {
-    // ---- 4. few: sorted, largest first, an entry per thread (bitonic)
-    const bool real = tid < have;
-    const float v = real ? to_f32(given_v[tid]) : 0.0f;
-    const int id = real ? given_i[tid] : -1;
-    u64 x = real ? ((u64)Key<T>::of(v) << 32) | (uint32_t)~(uint32_t)tid : 0;
-    int size = 32;
-    while (size < have) size <<= 1;
-    for (int len = 2; len <= size; len <<= 1)
-      for (int s = len >> 1; s; s >>= 1) {
-        u64 y;
-        if (s >= 32) {
-          __syncthreads();
-          sh.sorted[tid] = x;
-          __syncthreads();
-          y = sh.sorted[tid ^ s];
-        } else {
-          y = __shfl_xor_sync(kFull, x, s);
-        }
-        const bool first = (tid & s) == 0, down = (tid & len) == 0 || len == size;
-        x = first == down ? max(x, y) : min(x, y);
+  if (local && have <= kFewCap) {
+    // ---- 4. few: thread t has an entry; its rank and the weight before it by comparison with all
+    const int threads = (have + 31) & ~31;  // whole warps; they meet at barrier 1
+    if (tid < threads) {
+      auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); };
+      const bool real = tid < have;
+      const float v = real ? sh.few_v[tid] : 0.0f;
+      const int id = real ? sh.few_i[tid] : 0;
+      const float w = real ? weight(v) : 0.0f;
+      const u64 f = fixed(w);
+      const u64 x = ((u64)Key<T>::of(v) << 32) | (uint32_t)~(uint32_t)id;  // larger: ahead
+      if (real) {
+        sh.few_x[tid] = x;
+        sh.few_f[tid] = f;
       }
-    // thread t has the entry of rank t: prefixes by count, by weight, by the weight's share
-    const float w = real ? weight(Key<T>::value((uint32_t)(x >> 32))) : 0.0f;
-    const u64 f = fixed(w);
-    const bool in_k = real && (!by_k || tid < k);
-    const u64 incl = block_inclusive(in_k ? f : 0, sh.warp_sum);
-    if (by_k && by_p) {
-      if (tid == kSampThreads - 1) sh.exchange[2] = incl;
-      __syncthreads();
-      mass = sh.exchange[2];
+      meet();
+      int place = 0;
+      u64 before = 0;
+#pragma unroll 8
+      for (int j = 0; j < have; j++) {
+        const u64 ahead = (u64)0 - (u64)(sh.few_x[j] > x);  // all ones or 0
+        place -= (int)ahead;
+        before += sh.few_f[j] & ahead;
+      }
+      const bool in_k = real && (!by_k || place < k);
+      if (by_k && by_p) {  // the weight of what top-k keeps
+        if (real && place == min(k, have) - 1) sh.exchange[2] = before + f;
+        meet();
+        mass = sh.exchange[2];
+      }
+      const bool keep = in_k && (!by_p || place == 0 || (double)before < (double)top_p * (double)mass) && w >= min_p;
+      const u64 g = keep ? f : 0;
+      meet();
+      if (real) sh.few_f[tid] = g;
+      meet();
+      u64 total = 0, cdf = 0;
+#pragma unroll 8
+      for (int j = 0; j < have; j++) {
+        const u64 gj = sh.few_f[j];
+        total += gj;
+        cdf += gj & ((u64)0 - (u64)(sh.few_i[j] <= id));
+      }
+      const double target = (double)u * (double)total;
+      auto passed = [&](u64 c) { return (double)c > target || c >= total; };
+      if (g && passed(cdf) && !(cdf > g && passed(cdf - g))) finish(id, w, total);
     }
-    const bool keep = in_k && (!by_p || tid == 0 || (double)(incl - f) < (double)top_p * (double)mass) && w >= min_p;
-    // back in index order
-    __syncthreads();
-    if (real) sh.sorted[(uint32_t)~(uint32_t)x] = keep ? f : 0;
-    __syncthreads();
-    const u64 g = real ? sh.sorted[tid] : 0;
-    const u64 cdf = block_inclusive(g, sh.warp_sum);
-    if (tid == kSampThreads - 1) sh.exchange[3] = cdf;
-    __syncthreads();
-    const u64 total = sh.exchange[3];
-    const double target = (double)u * (double)total;
-    auto passed = [&](u64 c) { return (double)c > target || c >= total; };
-    if (g && passed(cdf) && !(cdf > g && passed(cdf - g))) finish(id, weight(v), total);
+    cl.barrier_wait();  // the others have read this CTA's count
     return;
   }
 
@@ -670,11 +769,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const __grid_
 template <typename T>
 cudaError_t launch(const SampleArgs& args, cudaStream_t s) {
   SampleArgs a = args;
-  // CTAs per row: as many as keep about 2,048 entries each, while the grid leaves SMs idle up to
-  // 16 a row; then 8 of which two fit an SM.
+  // CTAs per row: slices of which two fit an SM (76 KB beside the 36 KB of tables), so that one
+  // CTA's barriers and passes overlap another's; more, up to 16 and down to 2,048 entries each,
+  // while the rows leave SMs idle.
   int cluster = 1;
-  while (cluster < kMaxCluster && a.vocab > cluster * 4096 && (cluster < 8 || a.rows * cluster * 2 <= 2 * kAttnSms))
-    cluster *= 2;
+  while (cluster < 8 && (int64_t)a.vocab * (int)sizeof(T) > (int64_t)cluster * 76 * 1024) cluster *= 2;
+  while (cluster < kMaxCluster && a.vocab > cluster * 4096 && (int64_t)a.rows * cluster * 2 <= 2 * kAttnSms) cluster *= 2;
   const int align = 16 / (int)sizeof(T);
   a.slice = ((a.vocab + cluster - 1) / cluster + align - 1) / align * align;
   const size_t head = (sizeof(SampleShared) + 15) & ~(size_t)15;

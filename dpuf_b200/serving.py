@@ -212,7 +212,7 @@ def rope_append(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor, k:
         raise ValueError("seq and pos must have one entry a token")
     _check_table(page_table, dev)
     if out is None:
-        out = q.new_empty((n, n_q, hd))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, of q's shape and on its device")
     elif out.dtype not in _CODE:
@@ -274,7 +274,7 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
         _check(kv_len, "kv_len", _INT, dev, 1)
         raise ValueError("q_start must have one entry more than page_table has rows, kv_len as many")
     if out is None:
-        out = q.new_empty((n, n_q, hd))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError("out must be contiguous, of q's shape and on its device")
     elif out.dtype != q.dtype and out.dtype != _FLOAT:
@@ -328,8 +328,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | No
 
     values = (row_values(u, "u", _FLOAT), row_values(temperature, "temperature", _FLOAT),
               row_values(top_k, "top_k", _INT), row_values(top_p, "top_p", _FLOAT), row_values(min_p, "min_p", _FLOAT))
-    probs = u.new_empty(rows)
-    ids = probs.new_empty(rows, dtype=_INT)
+    probs = torch.empty_like(u)
+    ids = torch.empty_like(u, dtype=_INT)
     _call(_lib().dpuf_cuda_sample_rows, dev, logits.data_ptr(), code, logits.stride(0), rows, vocab,
           *values, ids.data_ptr(), probs.data_ptr())
     return ids, probs
