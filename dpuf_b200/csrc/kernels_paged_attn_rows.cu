@@ -70,7 +70,7 @@ DPUF_DEV float rest(float x) {
 
 template <int DP>
 struct RowsLay {
-  static constexpr int warps = DP == 256 ? 4 : 8;
+  static constexpr int warps = DP == 256 ? 2 : 4;  // two CTAs fit an SM: one joins while the other streams
   static constexpr int keys = 16 * warps;         // of a block
   static constexpr int stages = DP == 64 ? 6 : 3;
   static constexpr int half = 16 * DP * 2;        // bytes of a warp's keys (or values) of a block
@@ -80,7 +80,7 @@ struct RowsLay {
 };
 
 template <typename T, int DP, int kTerms>  // kTerms 1: queries of type T, else fp32
-__global__ void __launch_bounds__(RowsLay<DP>::warps * 32, 1)
+__global__ void __launch_bounds__(RowsLay<DP>::warps * 32, 2)
 paged_attention_rows_kernel(const __grid_constant__ AttnArgs p) {
   using Lay = RowsLay<DP>;
   constexpr int W = Lay::warps, kKeys = Lay::keys, S = Lay::stages;
@@ -387,7 +387,7 @@ template <typename T, int DP, int kTerms>
 cudaError_t launch(const AttnArgs& p, cudaStream_t s) {
   const cudaError_t e = smem_limit_once<paged_attention_rows_kernel<T, DP, kTerms>>(RowsLay<DP>::bytes);
   if (e != cudaSuccess) return e;
-  paged_attention_rows_kernel<T, DP, kTerms><<<kAttnSms, RowsLay<DP>::warps * 32, RowsLay<DP>::bytes, s>>>(p);
+  paged_attention_rows_kernel<T, DP, kTerms><<<kAttnSms * 2, RowsLay<DP>::warps * 32, RowsLay<DP>::bytes, s>>>(p);
   return cudaGetLastError();
 }
 
