@@ -70,14 +70,12 @@ DPUF_EXPORT int32_t dpuf_cuda_rope_append(const DpufRopeAppendArgs* args, void* 
   if (a.rotary_dim < 2 || a.rotary_dim % 2 || a.rotary_dim > a.kv.head_dim)
     return refuse(me, "rotary_dim must be even, at least 2 and at most head_dim");
   if (a.n_pos <= 0) return refuse(me, "empty rotary tables");
-  // Units of 16 dimensions move in 16-byte accesses (rope_append_kernel) where sizes and
-  // alignment allow; everything else goes pair by pair.
   const int b = type_bytes(a.dtype);
-  const bool vectors = a.kv.head_dim % 16 == 0 && a.rotary_dim % 16 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
-                       aligned(a.v, 16) && aligned(a.q_out, 16) && aligned(a.cos_tab, 16) && aligned(a.sin_tab, 16) &&
-                       a.q_stride[0] * b % 16 == 0 && a.q_stride[1] * b % 16 == 0 && a.k_stride[0] * b % 16 == 0 &&
-                       a.k_stride[1] * b % 16 == 0 && a.v_stride[0] * b % 16 == 0 && a.v_stride[1] * b % 16 == 0;
-  return finish(me, launch_rope_append(a, vectors, (cudaStream_t)stream));
+  const bool rows_aligned = aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.q_out, 16) &&
+                            aligned(a.cos_tab, 16) && aligned(a.sin_tab, 16) && a.q_stride[0] * b % 16 == 0 &&
+                            a.q_stride[1] * b % 16 == 0 && a.k_stride[0] * b % 16 == 0 &&
+                            a.k_stride[1] * b % 16 == 0 && a.v_stride[0] * b % 16 == 0 && a.v_stride[1] * b % 16 == 0;
+  return finish(me, launch_rope_append(a, rows_aligned, (cudaStream_t)stream));
 }
 
 DPUF_EXPORT int64_t dpuf_cuda_paged_attention_workspace(void) { return paged_attention_workspace(); }

@@ -97,7 +97,7 @@ DPUF_DEV void store4_as(void* p, size_t i, int dtype, float a, float b, float c,
 }
 
 // ---- launchers (arguments checked by the callers in ops_serving.cu)
-cudaError_t launch_rope_append(const DpufRopeAppendArgs& a, bool vectors, cudaStream_t s);
+cudaError_t launch_rope_append(const DpufRopeAppendArgs& a, bool aligned, cudaStream_t s);  // aligned: 16-byte accesses to rows
 cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t s);
 int64_t paged_attention_workspace();
 cudaError_t paged_attention_status(void* workspace, bool* gave_up, cudaStream_t s);

@@ -193,8 +193,8 @@ typedef struct DpufPagedKv {
  * pos[t].  The first rotary_dim (even) dimensions of each head of q and k are turned pair by
  * pair, (i, i + rotary_dim/2), or (2i, 2i + 1) if interleaved, with row pos[t] of the tables
  * cos_tab and sin_tab [n_pos][rotary_dim/2]:  (a, b) -> (a cos - b sin, b cos + a sin) in fp32,
- * rounded once.  The turned q goes to q_out [n_tokens][n_q][head_dim] (contiguous), the turned k
- * and v go to the cache.  dtype is that of q, k and v, out_dtype that of q_out.  A token with
+ * rounded once.  The turned q goes to q_out [n_tokens][n_q][head_dim] (contiguous; it may be q
+ * itself where q is contiguous and of out_dtype), the turned k and v go to the cache.  dtype is that of q, k and v, out_dtype that of q_out.  A token with
  * pos < 0 is padding (q_out gets zeros, nothing is stored); one with pos >= n_pos has no table
  * row (q_out gets NaN, nothing is stored); one whose page is not held is not stored.  Tokens of
  * one call that share a position race. */

@@ -96,7 +96,7 @@ def test_rope_append(types, shape, interleaved):
 
 
 def test_rope_append_unaligned_and_in_place():
-    """Rows that start off 16-byte boundaries go pair by pair; q may be turned in place."""
+    """Rows that start off 16-byte boundaries go element by element; q may be turned in place."""
     g = gen(3)
     n, hq, hkv, hd = 19, 4, 2, 64
     cache = serving.PagedCache.empty(4, hkv, 16, hd, F16)
@@ -111,7 +111,25 @@ def test_rope_append_unaligned_and_in_place():
     b = q.contiguous()
     serving.rope_append(cache, table, b, k.contiguous(), v.contiguous(), cos, sin, seq, pos, out=b)
     kb = cache.k_pages[[2] * 16 + [0] * (n - 16), :, [i % 16 for i in range(n)]]
-    assert torch.equal(a, b) and torch.equal(ka, kb)  # the two kernels do the same arithmetic
+    assert torch.equal(a, b) and torch.equal(ka, kb)  # the kernels do the same arithmetic
+
+
+@pytest.mark.parametrize("hd,rot", [(128, 128), (128, 36), (80, 20), (256, 250), (8, 8)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_append_in_place(hd, rot, interleaved):
+    """q turned in place equals q turned into a new tensor, with partners in other threads' runs too."""
+    g = gen(rot)
+    n, hq, hkv = 700, 6, 2
+    cache = serving.PagedCache.empty(50, hkv, 16, hd, F16)
+    table = torch.arange(50, dtype=INT, device="cuda")[None]
+    cos, sin = serving.rope_table(800, rot)
+    q, k, v = (normal(g, n, h, hd, dtype=F16) for h in (hq, hkv, hkv))
+    pos = torch.arange(n, dtype=INT, device="cuda")
+    want = serving.rope_append(cache, table, q, k, v, cos, sin, torch.zeros_like(pos), pos, interleaved)
+    for _ in range(5):
+        mine = q.clone()
+        serving.rope_append(cache, table, mine, k, v, cos, sin, torch.zeros_like(pos), pos, interleaved, out=mine)
+        assert torch.equal(mine, want)
 
 
 @pytest.mark.parametrize("rot", [64, 10])  # both kernels
