@@ -9,6 +9,9 @@
 // crosses a cut is computed in parts: each CTA leaves its part's running maximum, sum and
 // unnormalised output in the workspace, and the CTA that arrives last (a counter per item, no
 // waiting) joins the parts in the order of their keys, so results do not depend on timing.
+// An item counts kLead blocks more than it has, for what it costs beside them (queries, results,
+// the pipeline's filling): they stand before its first, and a run that ends in them leaves the
+// whole item to the next.
 //   part of an item that began in an earlier CTA: slot 2c; part that a later CTA goes on with:
 //   slot 2c + 1; the counter is that of the CTA in which the item begins.
 #pragma once
@@ -65,13 +68,22 @@ struct AttnCursor {
   AttnSeq seq;
   int s, head, tile, tiles;
   int blk0, n_blk;    // the item's key blocks
-  int at;             // block within the item
+  int at;             // place within the item, from its lead on
   long long begin;    // the item's first block in the sequence of all
 };
 
-template <int BM, int BN>
+// The blocks [*from, *to) of the cursor's item that a run with `left` places takes, maybe none.
+template <int kLead>
+DPUF_DEV void attn_take(const AttnCursor& c, int& left, int* from, int* to) {
+  const int end = min(c.n_blk + kLead, c.at + left);
+  left -= end - c.at;
+  *from = max(c.at - kLead, 0);
+  *to = max(end - kLead, 0);
+}
+
+template <int BM, int BN, int kLead = 0>
 DPUF_DEV void attn_next_item(const AttnArgs& p, AttnCursor& c) {
-  c.begin += c.n_blk;
+  c.begin += c.n_blk + kLead;
   c.at = 0;
   if (++c.tile == c.tiles) {
     c.tile = 0;
@@ -102,19 +114,19 @@ struct AttnRun {  // this CTA's run of key blocks
 
 // Key blocks of one KV head of each lane's sequence.  A sequence of many tiles is shared by the
 // lanes (a prompt of 2,048 tokens has up to 128, which one thread would walk for microseconds).
-template <int BM, int BN>
+template <int BM, int BN, int kLead>
 DPUF_DEV long long attn_costs(const AttnArgs& p, const AttnSeq& q) {
   const int lane = threadIdx.x & 31, tiles = attn_tiles<BM>(p, q);
   long long cost = 0;
   int b0;
   unsigned many = __ballot_sync(kFull, tiles > 2);
   if (tiles <= 2)
-    for (int t = 0; t < tiles; t++) cost += attn_tile_blocks<BM, BN>(p, q, t, &b0);
+    for (int t = 0; t < tiles; t++) cost += attn_tile_blocks<BM, BN>(p, q, t, &b0) + kLead;
   for (; many; many &= many - 1) {
     const int j = __ffs(many) - 1;
     const AttnSeq o{__shfl_sync(kFull, q.q0, j), __shfl_sync(kFull, q.qn, j), __shfl_sync(kFull, q.kv, j)};
     long long c = 0;
-    for (int t = lane, n = attn_tiles<BM>(p, o); t < n; t += 32) c += attn_tile_blocks<BM, BN>(p, o, t, &b0);
+    for (int t = lane, n = attn_tiles<BM>(p, o); t < n; t += 32) c += attn_tile_blocks<BM, BN>(p, o, t, &b0) + kLead;
 #pragma unroll
     for (int i = 16; i; i >>= 1) c += __shfl_xor_sync(kFull, c, i);
     if (lane == j) cost = c;
@@ -133,14 +145,14 @@ DPUF_DEV long long attn_scan(long long v) {  // inclusive, over the warp
 
 // All threads of the CTA call this together.  A warp adds up a run of sequences, 32 at a time; the
 // warp in whose run the CTA's first block lies finds it.
-template <int BM, int BN>
+template <int BM, int BN, int kLead = 0>
 DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   const int per = (p.a.n_seqs + nw - 1) / nw;
   const int s0 = min(warp * per, p.a.n_seqs), s1 = min(s0 + per, p.a.n_seqs);
   auto seq_of = [&](int s) { return s + lane < s1 ? attn_seq(p, s + lane) : AttnSeq{0, 0, 0}; };
   long long mine = 0;
-  for (int s = s0; s < s1; s += 32) mine += attn_costs<BM, BN>(p, seq_of(s));
+  for (int s = s0; s < s1; s += 32) mine += attn_costs<BM, BN, kLead>(p, seq_of(s));
 #pragma unroll
   for (int i = 16; i; i >>= 1) mine += __shfl_xor_sync(kFull, mine, i);
   mine *= p.a.kv.n_kv;
@@ -159,7 +171,7 @@ DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas
     for (int s = s0;; s += 32) {
       AttnCursor c;
       c.seq = seq_of(s);
-      const long long k = attn_costs<BM, BN>(p, c.seq), end = at + attn_scan(k * p.a.kv.n_kv);
+      const long long k = attn_costs<BM, BN, kLead>(p, c.seq), end = at + attn_scan(k * p.a.kv.n_kv);
       const unsigned in = __ballot_sync(kFull, b < end);
       if (!in) {
         at = __shfl_sync(kFull, end, 31);
@@ -175,12 +187,13 @@ DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas
       c.tiles = attn_tiles<BM>(p, c.seq);
       for (int t0 = 0;; t0 += 32) {  // 32 tiles at a time
         c.n_blk = t0 + lane < c.tiles ? attn_tile_blocks<BM, BN>(p, c.seq, t0 + lane, &c.blk0) : 0;
-        const long long tile_end = at + attn_scan(c.n_blk);
+        const int places = t0 + lane < c.tiles ? c.n_blk + kLead : 0;
+        const long long tile_end = at + attn_scan(places);
         const unsigned hit = __ballot_sync(kFull, b < tile_end);
         if (hit) {
           if (lane == __ffs(hit) - 1) {
             c.tile = t0 + lane;
-            c.begin = tile_end - c.n_blk;
+            c.begin = tile_end - places;
             c.at = (int)(b - c.begin);
             sh.start = c;
           }
@@ -196,7 +209,7 @@ DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas
   return r;
 }
 
-// The CTA that holds block x of all.
+// The CTA that holds place x of all.
 DPUF_DEV int attn_cta_of(const AttnRun& r, long long x) { return (int)(((x + 1) * r.ctas - 1) / r.total); }
 
 // Cache offset (elements) of head 0, row 0 of the page that holds position j of sequence s, or -1.

@@ -47,6 +47,8 @@ constexpr int kKeys = 64;             // of a block
 constexpr int kItemRows = 2 * kTile;
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kQueryWarp = 11;  // kMmaWarp + i: tile i
 constexpr int kThreads = 384;
+// What an item costs beside its blocks, in blocks (four prompts of 2,048: 178 us at 0, 167 at 2, 168 at 3, 174 at 5).
+constexpr int kLead = 2;
 // The weights carry a factor 2^7, and so does their sum: at most 2^15, which fp16 holds, while the
 // small ones of a long context keep their bits.
 constexpr float kLift = 7.0f;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     abort_sh = 0;
   }
   fence_before();
-  AttnRun run = attn_locate<kItemRows, kKeys>(p, share, blockIdx.x, gridDim.x);
+  AttnRun run = attn_locate<kItemRows, kKeys, kLead>(p, share, blockIdx.x, gridDim.x);
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_sh;
@@ -296,9 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     unsigned it = 0;  // blocks requested so far
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
-      const int from = c.at, to = min(c.n_blk, c.at + left);
-      left -= to - from;
-      int lo, hi;
+      int from, to, lo, hi;
+      attn_take<kLead>(c, left, &from, &to);
       item_span(p, c.seq, c.tile, &lo, &hi);
       auto page_of = [&](int b) {  // of this lane's box
         const int j = (c.blk0 + b) * kKeys + lane * box;
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         }
         return page;
       };
-      int page = page_of(from);
+      int page = from < to ? page_of(from) : 0;
       for (int b = from; ok && b < to; b++, it++) {
         const int next = b + 1 < to ? page_of(b + 1) : 0;
         const int slot = it % S;
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         copy(&args.v_map, &v_full[slot], sm + Lay::v + slot * Lay::block);
         page = next;
       }
-      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+      if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
     }
     if (!ok)  // nothing in flight at exit (waits of at most 2 s each; a value block may be missing)
       for (unsigned i = it > S ? it - S : 0; i < it; i++) {
@@ -353,8 +354,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     const int ch = lane % kCh;
     const bool in = ch * 8 < p.a.kv.head_dim;
     bool ok = true;
-    for (int left = run.n, seg = 0; ok && left > 0; seg++) {
-      left -= min(c.n_blk, c.at + left) - c.at;
+    for (int left = run.n, seg = 0; ok && left > 0;) {
+      int from, to;
+      attn_take<kLead>(c, left, &from, &to);
+      if (from == to) {
+        if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
+        continue;
+      }
       if (!(ok = warp_wait(&q_empty[seg & 1], (seg >> 1 & 1) ^ 1, give))) break;
       const int total = c.seq.qn * p.group, r0 = c.tile * kItemRows;
       const uint32_t dst = su32(sm + Lay::q + (seg & 1) * 2 * Lay::tile);
@@ -376,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         } else {
           bar_arrive(&q_full[seg & 1]);
         }
-        if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+        seg++;
+        if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
         continue;
       }
       const char* const base = (const char*)p.a.q + ch * 16;
@@ -400,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         }
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(su32(&q_full[seg & 1])) : "memory");
-      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+      seg++;
+      if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight at exit
   } else if (warp >= kMmaWarp) {
@@ -415,9 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     unsigned seg = 0, blocks = 0;     // items, and blocks of this tile so far
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
-      const int from = c.at, to = min(c.n_blk, c.at + left), n = to - from;
-      left -= n;
-      int lo, hi;
+      int from, to, lo, hi;
+      attn_take<kLead>(c, left, &from, &to);
+      const int n = to - from;
+      if (n == 0) {
+        if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
+        continue;
+      }
       item_span(p, c.seq, c.tile, &lo, &hi);
       const bool mine = w == 0 || c.seq.qn * p.group - c.tile * kItemRows > kTile;
       const uint64_t dq = dq0 + (uint64_t)((seg & 1) * (2 * Lay::tile >> 4));
@@ -485,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       }
       seg++;
       base += n;
-      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+      if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
     }
   } else {
     // ================================================================ softmax: tile w, this thread's row
@@ -507,15 +519,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     bool ok = true;
     auto wg_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); };
     for (int left = run.n; ok && left > 0;) {
-      const int from = c.at, to = min(c.n_blk, c.at + left), n = to - from;
-      left -= n;
+      int from, to;
+      attn_take<kLead>(c, left, &from, &to);
+      const int n = to - from;
+      if (n == 0) {
+        if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
+        continue;
+      }
       const int total = c.seq.qn * p.group, r0 = c.tile * kItemRows + w * kTile;
       unsigned char* const qs = sm + Lay::q + ((seg & 1) * 2 + w) * Lay::tile;  // free once the last scores are in
       uint64_t* const q_done = &q_empty[seg & 1];
       seg++;
       if (w == 1 && r0 >= total) {  // one tile only
         if (lane == 0) bar_arrive(q_done);
-        if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+        if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
         continue;
       }
       const int r = r0 + t;
@@ -607,8 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           for (int e = 0; e < 32; e++)  // [dim][row]: a warp's rows are adjacent
             parts.o[(slot * DP + 32 * i + e) * kItemRows + pr] = __uint_as_float(o[e]);
         }
-        c0 = attn_cta_of(run, c.begin);
-        c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
+        c0 = attn_cta_of(run, c.begin + kLead);
+        c1 = attn_cta_of(run, c.begin + kLead + c.n_blk - 1);
         __threadfence();
         wg_sync();
         if (t == 0) flag_sh[w] = attn_arrive(parts.count + 2 * c0 + w, c1 - c0 + 1);
@@ -725,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       __syncwarp();
       if (lane == 0 && !pending) bar_arrive(q_done);
       fence_before();  // O is read: the next item's products may overwrite it once its P arrives
-      if (left > 0) attn_next_item<kItemRows, kKeys>(p, c);
+      if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // nothing in flight at exit
   }
