@@ -545,23 +545,30 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
   };
   // Entries with keys in [lo, hi] into bins of 2^shift keys from the top, and the bin in which the
   // count (by_count) or the weight, from the sums above, reaches the target.
+  // (top-p's first range is top-k's: its histogram is kept where top-k needed no other.)
+  uint32_t built_lo = 1, built_hi = 0;
   auto level = [&](uint32_t lo, uint32_t hi, int shift, bool by_count, const Found above, uint32_t k_target,
                    double p_target) {
+    const bool again = lo == built_lo && hi == built_hi;
+    built_lo = lo;
+    built_hi = hi;
     __syncthreads();
-    for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = sh.m0[b] = sh.m1[b] = sh.m2[b] = 0;
+    if (!again)
+      for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = sh.m0[b] = sh.m1[b] = sh.m2[b] = 0;
     if (tid == 0) sh.found = Found{-1, 0, 0, 0, 0};
     __syncthreads();
-    for (int i = tid; i < dn; i += kSampThreads) {
+#pragma unroll 4
+    for (int i = tid; i < (again ? 0 : dn); i += kSampThreads) {
       const float v = value(i);
       const uint32_t kv = Key<T>::of(v);
-      if (kv < lo || kv > hi) continue;
-      const u64 f = fixed(weight(v));
-      if (!f) continue;
-      const int b = (int)((hi - kv) >> shift);
-      atomicAdd(&sh.count[b], 1u);
-      atomicAdd(&sh.m0[b], (uint32_t)f & 0x7FFF);
-      atomicAdd(&sh.m1[b], (uint32_t)(f >> 15) & 0x7FFF);
-      atomicAdd(&sh.m2[b], (uint32_t)(f >> 30));
+      const u64 f = kv < lo || kv > hi ? 0 : fixed(weight(v));
+      if (f) {
+        const int b = (int)((hi - kv) >> shift);
+        atomicAdd(&sh.count[b], 1u);
+        atomicAdd(&sh.m0[b], (uint32_t)f & 0x7FFF);
+        atomicAdd(&sh.m1[b], (uint32_t)(f >> 15) & 0x7FFF);
+        atomicAdd(&sh.m2[b], (uint32_t)(f >> 30));
+      }
     }
     if (local) {
       __syncthreads();
@@ -586,45 +593,47 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
       return sh.found;
     }
     const int seg = kBins / R;
-    cl.sync();
-    for (int i = tid; i < 4 * seg; i += kSampThreads) {  // four threads a bin, each some of the CTAs
-      const int g = rank * seg + (i >> 2);
-      uint32_t c = 0;
-      u64 f = 0;
+    if (!again) {
+      cl.sync();
+      for (int i = tid; i < 4 * seg; i += kSampThreads) {  // four threads a bin, each some of the CTAs
+        const int g = rank * seg + (i >> 2);
+        uint32_t c = 0;
+        u64 f = 0;
 #pragma unroll 4
-      for (int r = i & 3; r < R; r += 4) {
-        const SampleShared* o = of(r);
-        c += o->count[g];
-        f += (u64)o->m0[g] + ((u64)o->m1[g] << 15) + ((u64)o->m2[g] << 30);
-      }
+        for (int r = i & 3; r < R; r += 4) {
+          const SampleShared* o = of(r);
+          c += o->count[g];
+          f += (u64)o->m0[g] + ((u64)o->m1[g] << 15) + ((u64)o->m2[g] << 30);
+        }
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        c += __shfl_xor_sync(kFull, c, o);
-        f += __shfl_xor_sync(kFull, f, o);
+        for (int o = 1; o < 4; o <<= 1) {
+          c += __shfl_xor_sync(kFull, c, o);
+          f += __shfl_xor_sync(kFull, f, o);
+        }
+        if ((i & 3) == 0) {
+          sh.bin_count[i >> 2] = c;
+          sh.bin_mass[i >> 2] = f;
+        }
       }
-      if ((i & 3) == 0) {
-        sh.bin_count[i >> 2] = c;
-        sh.bin_mass[i >> 2] = f;
-      }
-    }
-    __syncthreads();
-    if (tid < 32) {
-      u64 cs = 0, ms = 0;
-      for (int b = lane; b < seg; b += 32) {
-        cs += sh.bin_count[b];
-        ms += sh.bin_mass[b];
-      }
+      __syncthreads();
+      if (tid < 32) {
+        u64 cs = 0, ms = 0;
+        for (int b = lane; b < seg; b += 32) {
+          cs += sh.bin_count[b];
+          ms += sh.bin_mass[b];
+        }
 #pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        cs += __shfl_xor_sync(kFull, cs, o);
-        ms += __shfl_xor_sync(kFull, ms, o);
+        for (int o = 16; o; o >>= 1) {
+          cs += __shfl_xor_sync(kFull, cs, o);
+          ms += __shfl_xor_sync(kFull, ms, o);
+        }
+        if (lane == 0) {
+          sh.seg_count = (uint32_t)cs;
+          sh.seg_mass = ms;
+        }
       }
-      if (lane == 0) {
-        sh.seg_count = (uint32_t)cs;
-        sh.seg_mass = ms;
-      }
+      cl.sync();
     }
-    cl.sync();
     if (tid < 32) {
       const u64 c0 = lane < R ? of(lane)->seg_count : 0, f0 = lane < R ? of(lane)->seg_mass : 0;
       const u64 ci = warp_inclusive(c0) + above.above, fi = warp_inclusive(f0) + above.mass_above;
