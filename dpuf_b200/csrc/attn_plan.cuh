@@ -81,6 +81,23 @@ DPUF_DEV void attn_take(const AttnCursor& c, int& left, int* from, int* to) {
   *to = max(end - kLead, 0);
 }
 
+// The order in which a run takes its `n` blocks from `from` on of the cursor's item: from a block
+// that stands where the run does (`done` places in, modulo a run's length), then round.  The CTAs
+// that work on a head's tiles are then at the same keys at the same time, and read them from
+// memory once (512 tokens over 33,280 positions: 167 MB instead of 497, of 145).
+struct AttnOrder {
+  int from, n, first;
+  DPUF_DEV AttnOrder(const AttnCursor& c, int from_, int n_, int done, int length) : from(from_), n(n_) {
+    int d = (done - c.blk0 - from_) % length;
+    if (d < 0) d += length;
+    first = d < n_ ? d : 0;
+  }
+  DPUF_DEV int block(int i) const {
+    const int k = i + first;
+    return from + (k < n ? k : k - n);
+  }
+};
+
 template <int BM, int BN, int kLead = 0>
 DPUF_DEV void attn_next_item(const AttnArgs& p, AttnCursor& c) {
   c.begin += c.n_blk + kLead;

@@ -291,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
   fence_after();
   const uint32_t tmem = tmem_sh;
   AttnCursor& c = run.cur;
+  const int length = max((int)(run.total / max(run.ctas, 1)), 1);  // of a run, as all CTAs see it
 
   if (warp == kLoadWarp) {
     // ================================================================ TMA
@@ -299,7 +300,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
       int from, to, lo, hi;
+      const int done = run.n - left;
       attn_take<kLead>(c, left, &from, &to);
+      const int n = to - from;
+      const AttnOrder order(c, from, n, done, length);
       item_span(p, c.seq, c.tile, &lo, &hi);
       auto page_of = [&](int b) {  // of this lane's box
         const int j = (c.blk0 + b) * kKeys + lane * box;
@@ -310,9 +314,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         }
         return page;
       };
-      int page = from < to ? page_of(from) : 0;
-      for (int b = from; ok && b < to; b++, it++) {
-        const int next = b + 1 < to ? page_of(b + 1) : 0;
+      int page = n ? page_of(order.block(0)) : 0;
+      for (int i = 0; ok && i < n; i++, it++) {
+        const int b = order.block(i), next = i + 1 < n ? page_of(order.block(i + 1)) : 0;
         const int slot = it % S;
         const unsigned par = (it / S & 1) ^ 1;
         const int row = ((c.blk0 + b) * kKeys + lane * box) & (p.a.kv.page_size - 1);
@@ -424,8 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
       int from, to, lo, hi;
+      const int done = run.n - left;
       attn_take<kLead>(c, left, &from, &to);
       const int n = to - from;
+      const AttnOrder order(c, from, n, done, length);
       if (n == 0) {
         if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
         continue;
@@ -469,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           const unsigned g = base + b, e = blocks + b;
           const int slot = g % S;
           if (!(ok = warp_wait(&v_full[slot], g / S & 1, give))) break;
-          const int j0 = (c.blk0 + from + b) * kKeys;
+          const int j0 = (c.blk0 + order.block(b)) * kKeys;
           const int z0 = max(lo - j0, 0), z1 = min(hi - j0, kKeys);  // rows that the item sees
           if (z0 > 0 || z1 < kKeys) {  // (both tiles' warps write these zeros)
             unsigned char* v = sm + Lay::v + slot * Lay::block;
@@ -520,8 +526,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     auto wg_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); };
     for (int left = run.n; ok && left > 0;) {
       int from, to;
+      const int done = run.n - left;
       attn_take<kLead>(c, left, &from, &to);
       const int n = to - from;
+      const AttnOrder order(c, from, n, done, length);
       if (n == 0) {
         if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
         continue;
@@ -542,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       if (live) attn_span(p, c.seq, tok, tok, &lo, &hi);
       float m = -CUDART_INF_F, l = 0.0f;  // m: the maximum that the weights refer to
       for (int b = 0; b < n; b++, blocks++) {
-        const int j0 = (c.blk0 + from + b) * kKeys, h = blocks & 1;
+        const int j0 = (c.blk0 + order.block(b)) * kKeys, h = blocks & 1;
         if (!(ok = warp_wait(&s_full[w][h], blocks >> 1 & 1, give))) break;
         fence_after();
         uint32_t s[kKeys];
