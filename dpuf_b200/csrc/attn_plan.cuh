@@ -119,7 +119,8 @@ DPUF_DEV void attn_next_item(const AttnArgs& p, AttnCursor& c) {
 struct AttnShare {  // in shared memory
   AttnCursor start;
   long long total;
-  long long warp_sum[32];
+  long long warp_sum[12];  // of the CTA's warps
+  int warp_items[12];
 };
 
 struct AttnRun {  // this CTA's run of key blocks
@@ -160,25 +161,42 @@ DPUF_DEV long long attn_scan(long long v) {  // inclusive, over the warp
   return v;
 }
 
+// Fewer CTAs than there are, where an item of n blocks would be cut into more than sqrt(n kJoin)
+// parts: a part costs the CTA that joins them about 1 / kJoin of a block's time, one after the other.
+//
 // All threads of the CTA call this together.  A warp adds up a run of sequences, 32 at a time; the
 // warp in whose run the CTA's first block lies finds it.
 template <int BM, int BN, int kLead = 0>
-DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas) {
+DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas, float join) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   const int per = (p.a.n_seqs + nw - 1) / nw;
   const int s0 = min(warp * per, p.a.n_seqs), s1 = min(s0 + per, p.a.n_seqs);
   auto seq_of = [&](int s) { return s + lane < s1 ? attn_seq(p, s + lane) : AttnSeq{0, 0, 0}; };
-  long long mine = 0;
-  for (int s = s0; s < s1; s += 32) mine += attn_costs<BM, BN, kLead>(p, seq_of(s));
+  long long mine = 0, items = 0;
+  for (int s = s0; s < s1; s += 32) {
+    const AttnSeq q = seq_of(s);
+    mine += attn_costs<BM, BN, kLead>(p, q);
+    items += attn_tiles<BM>(p, q);
+  }
 #pragma unroll
-  for (int i = 16; i; i >>= 1) mine += __shfl_xor_sync(kFull, mine, i);
+  for (int i = 16; i; i >>= 1) {
+    mine += __shfl_xor_sync(kFull, mine, i);
+    items += __shfl_xor_sync(kFull, items, i);
+  }
   mine *= p.a.kv.n_kv;
-  if (lane == 0) sh.warp_sum[warp] = mine;
+  if (lane == 0) {
+    sh.warp_sum[warp] = mine;
+    sh.warp_items[warp] = (int)min(items * p.a.kv.n_kv, (long long)0x7FFFFFF);
+  }
   __syncthreads();
   const long long sums = attn_scan(lane < nw ? sh.warp_sum[lane] : 0);
   AttnRun r;
   r.total = __shfl_sync(kFull, sums, 31);
-  r.ctas = (int)min((long long)ctas, r.total);
+  items = lane < nw ? sh.warp_items[lane] : 0;
+#pragma unroll
+  for (int i = 16; i; i >>= 1) items += __shfl_xor_sync(kFull, items, i);
+  const float parts = items ? fmaxf(sqrtf((float)r.total / (float)items * join), 1.0f) : 0.0f;
+  r.ctas = (int)min(min((long long)ctas, r.total), (long long)(parts * (float)items));
   r.n = 0;
   if (cta >= r.ctas) return r;  // the whole CTA
   const long long b = r.total * cta / r.ctas, e = r.total * (cta + 1) / r.ctas;

@@ -29,6 +29,7 @@ DPUF_DEV float ex2(float x) {
 // (row = tid / 16, x = tid % 16) has the scores of keys x and x + 16 and the output's dimensions
 // 4 x + 64 i of its row; a row's 16 threads are half a warp.
 constexpr int kGenRows = 16, kGenKeys = 32, kGenThreads = 256;
+constexpr float kJoin = 8.0f;
 
 template <typename TK, int DP>  // DP: head_dim rounded up to 64, 128 or 256
 __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const __grid_constant__ AttnArgs p) {
@@ -42,7 +43,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
   __shared__ int flag;
   const int tid = threadIdx.x, row = tid >> 4, x = tid & 15;
   const int hd = p.a.kv.head_dim;
-  AttnRun run = attn_locate<kGenRows, kGenKeys>(p, share, blockIdx.x, gridDim.x);
+  AttnRun run = attn_locate<kGenRows, kGenKeys>(p, share, blockIdx.x, gridDim.x, kJoin);
   if (run.n == 0) return;
   const AttnParts<kGenRows, DP> parts(p.a.workspace, gridDim.x);
   AttnCursor& c = run.cur;

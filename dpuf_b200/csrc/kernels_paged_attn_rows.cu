@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kRows = 16;
 constexpr float kLift = 12.0f;
+constexpr float kJoin = 8.0f;
 
 DPUF_DEV uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 DPUF_DEV float ex2(float x) {
@@ -92,7 +93,7 @@ paged_attention_rows_kernel(const __grid_constant__ AttnArgs p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hd = p.a.kv.head_dim;
   const AttnParts<kRows, DP> parts(p.a.workspace, gridDim.x);
-  AttnRun run = attn_locate<kRows, kKeys>(p, share, blockIdx.x, gridDim.x);
+  AttnRun run = attn_locate<kRows, kKeys>(p, share, blockIdx.x, gridDim.x, kJoin);
   if (run.n == 0) return;
 
   // ---- the warp's stream of keys and values

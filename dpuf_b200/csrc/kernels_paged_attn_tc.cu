@@ -49,6 +49,7 @@ constexpr int kLoadWarp = 8, kMmaWarp = 9, kQueryWarp = 11;  // kMmaWarp + i: ti
 constexpr int kThreads = 384;
 // What an item costs beside its blocks, in blocks (four prompts of 2,048: 178 us at 0, 167 at 2, 168 at 3, 174 at 5).
 constexpr int kLead = 2;
+constexpr float kJoin = 0.33f;
 // The weights carry a factor 2^7, and so does their sum: at most 2^15, which fp16 holds, while the
 // small ones of a long context keep their bits.
 constexpr float kLift = 7.0f;
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
   constexpr int S = Lay::stages;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t k_full[S], k_empty[S], v_full[S], v_empty[S];
-  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty[2], drained[2], s_full[2][2], p_full[2][2], pv_done[2][2];
   __shared__ AttnShare share;
   __shared__ uint32_t tmem_sh;
   __shared__ int abort_sh, flag_sh[2];
@@ -276,6 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     for (int i = 0; i < 2; i++) {
       bar_init(&q_full[i], 32);
       bar_init(&q_empty[i], 8);
+      bar_init(&drained[i], 1);
       for (int h = 0; h < 2; h++) {
         bar_init(&s_full[i][h], 1);
         bar_init(&p_full[i][h], kTile);
@@ -286,17 +288,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     abort_sh = 0;
   }
   fence_before();
-  AttnRun run = attn_locate<kItemRows, kKeys, kLead>(p, share, blockIdx.x, gridDim.x);
+  AttnRun run = attn_locate<kItemRows, kKeys, kLead>(p, share, blockIdx.x, gridDim.x, kJoin);
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_sh;
   AttnCursor& c = run.cur;
   const int length = max((int)(run.total / max(run.ctas, 1)), 1);  // of a run, as all CTAs see it
+  unsigned it = 0, asked = 0;  // key and value blocks, items' queries requested so far (by their warps)
 
   if (warp == kLoadWarp) {
     // ================================================================ TMA
     const int box = min(p.a.kv.page_size, kKeys), boxes = kKeys / box;
-    unsigned it = 0;  // blocks requested so far
     bool ok = true;
     for (int left = run.n; ok && left > 0;) {
       int from, to, lo, hi;
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         if (!(ok = warp_wait(&k_empty[slot], par, give))) break;
         copy(&args.k_map, &k_full[slot], sm + Lay::k + slot * Lay::block);
         if (!(ok = warp_wait(&v_empty[slot], par, give))) {
-          it++;
+          it++;  // (its keys are on the way)
           break;
         }
         copy(&args.v_map, &v_full[slot], sm + Lay::v + slot * Lay::block);
@@ -345,20 +347,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       }
       if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
     }
-    if (!ok)  // nothing in flight at exit (waits of at most 2 s each; a value block may be missing)
-      for (unsigned i = it > S ? it - S : 0; i < it; i++) {
-        const unsigned long long t0 = gtimer();
-        while (!bar_try(&k_full[i % S], i / S & 1) && gtimer() - t0 < kWaitNs) {}
-        const unsigned long long t1 = gtimer();
-        while (!bar_try(&v_full[i % S], i / S & 1) && gtimer() - t1 < kWaitNs / 100) {}
-      }
   } else if (warp == kQueryWarp) {
     // ================================================================ queries, an item ahead
     constexpr int kCh = DP / 8, kStep = 32 / kCh;  // 16-byte chunks of a row, rows of a pass
     const int ch = lane % kCh;
     const bool in = ch * 8 < p.a.kv.head_dim;
     bool ok = true;
-    for (int left = run.n, seg = 0; ok && left > 0;) {
+    for (int left = run.n; ok && left > 0;) {
+      const unsigned seg = asked;
       int from, to;
       attn_take<kLead>(c, left, &from, &to);
       if (from == to) {
@@ -386,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         } else {
           bar_arrive(&q_full[seg & 1]);
         }
-        seg++;
+        asked++;
         if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
         continue;
       }
@@ -411,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         }
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(su32(&q_full[seg & 1])) : "memory");
-      seg++;
+      asked++;
       if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight at exit
@@ -458,6 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           mma_commit(&k_empty[slot]);
         }
       };
+      // in both tiles' warps, also for an item of one tile: a wait for a phase is only good if the
+      // one before it was seen
+      ok = warp_wait(&q_full[seg & 1], seg >> 1 & 1, give);
       if (!mine) {  // the other tile alone: this one's share of the ring's bookkeeping
         for (int b = 0; ok && b < n; b++) {
           const unsigned g = base + b;
@@ -467,8 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           if (lane == 0) bar_arrive(&v_empty[g % S]);
         }
       } else {
-        ok = warp_wait(&q_full[seg & 1], seg >> 1 & 1, give);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the copies are generic writes
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the copies may be generic writes
         if (ok) scores(0);
         if (ok && n > 1) scores(1);
         for (int b = 0; ok && b < n; b++) {
@@ -538,8 +536,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
       unsigned char* const qs = sm + Lay::q + ((seg & 1) * 2 + w) * Lay::tile;  // free once the last scores are in
       uint64_t* const q_done = &q_empty[seg & 1];
       seg++;
-      if (w == 1 && r0 >= total) {  // one tile only
-        if (lane == 0) bar_arrive(q_done);
+      const bool alone = total - c.tile * kItemRows <= kTile;  // one tile only
+      if (w == 1 && alone) {  // (tile 0 arrives on q_done for both, when the item is done)
+        stored();
         if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
         continue;
       }
@@ -748,7 +747,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         else write(std::false_type());
       }
       __syncwarp();
-      if (lane == 0 && !pending) bar_arrive(q_done);
+      if (lane == 0) {
+        if (alone) bar_arrive(q_done);
+        if (!pending) bar_arrive(q_done);
+      }
       fence_before();  // O is read: the next item's products may overwrite it once its P arrives
       if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
     }
@@ -757,6 +759,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
   fence_before();
   __syncthreads();
   fence_after();
+  if (abort_sh) {  // nothing in flight at exit: bounded waits for the copies and the products asked for
+    auto settle = [&](uint64_t* bar, unsigned par) {
+      const unsigned long long t0 = gtimer();
+      while (!bar_try(bar, par) && gtimer() - t0 < kWaitNs / 100) {}
+    };
+    if (warp == kLoadWarp)
+      for (unsigned i = it > S ? it - S : 0; i < it; i++) {
+        settle(&k_full[i % S], i / S & 1);
+        settle(&v_full[i % S], i / S & 1);
+      }
+    if (warp == kQueryWarp)
+      for (unsigned i = asked > 2 ? asked - 2 : 0; i < asked; i++) settle(&q_full[i & 1], i >> 1 & 1);
+    if (warp >= kMmaWarp && warp < kQueryWarp) {
+      if (elect_one()) mma_commit(&drained[warp - kMmaWarp]);
+      settle(&drained[warp - kMmaWarp], 0);
+    }
+    __syncthreads();
+  }
   if (warp == kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }

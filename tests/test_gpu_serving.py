@@ -154,45 +154,50 @@ def test_rope_append_out_of_range(rot):
 
 # ---------------------------------------------------------------- paged_attention
 def attention64(cache, table, q, q_start, kv_len, scale, causal, window):
-    """Plain attention in 64 bits, token by token, and a bound on the error of each output."""
+    """Plain attention in 64 bits, sequence by sequence, and a bound on the error of each output."""
     page, hkv = cache.page_size, cache.n_kv
     n, hq, hd = q.shape
     out = torch.zeros(n, hq, hd, dtype=torch.float64, device="cuda")
     bound = torch.zeros_like(out)
     for s in range(len(kv_len)):
         first, end, total = q_start[s], q_start[s + 1], kv_len[s]
-        for t in range(first, end):
-            p = total - (end - first) + (t - first)
-            hi = min(total, p + 1) if causal else total
-            lo = max(0, p - window + 1) if window else 0
-            if hi <= lo:
-                continue
-            at = torch.arange(lo, hi, device="cuda")
-            pages, rows = table[s, at // page].long(), at % page
-            k = cache.k_pages[pages, :, rows].double().repeat_interleave(hq // hkv, 1)
-            v = cache.v_pages[pages, :, rows].double().repeat_interleave(hq // hkv, 1)
-            x = q[t].double()
-            w = torch.softmax(torch.einsum("hd,jhd->hj", x, k) * scale, 1)
-            out[t] = torch.einsum("hj,jhd->hd", w, v)
-            bound[t] = attention_bound(x, k, v, w, scale, cache.dtype if q.dtype != F32 else F32, q.dtype)
+        if first == end or total == 0:
+            continue
+        p = torch.arange(total - (end - first), total, device="cuda")[:, None]
+        low = max(0, total - (end - first) - window + 1) if window else 0  # no token of it sees less
+        at = torch.arange(low, total, device="cuda")
+        sees = at[None] <= p if causal else torch.ones(end - first, total - low, dtype=torch.bool, device="cuda")
+        if window:
+            sees = sees & (at[None] > p - window)
+        pages, rows = table[s, at // page].long(), at % page
+        k = cache.k_pages[pages, :, rows].double().repeat_interleave(hq // hkv, 1)
+        v = cache.v_pages[pages, :, rows].double().repeat_interleave(hq // hkv, 1)
+        x = q[first:end].double()
+        score = (torch.einsum("thd,jhd->htj", x, k) * scale).masked_fill(~sees, -math.inf)
+        w = torch.softmax(score, 2).nan_to_num(0.0)  # (a token that sees nothing)
+        out[first:end] = torch.einsum("htj,jhd->thd", w, v)
+        bound[first:end] = attention_bound(x, k, v, w, sees, scale, cache.dtype if q.dtype != F32 else F32, q.dtype)
     return out, bound
 
 
-def attention_bound(x, k, v, w, scale, p_type, out_type):
+def attention_bound(x, k, v, w, sees, scale, p_type, out_type):
     """A score is a sum of head_dim fp32 products scaled by one more: off by e <= (head_dim + 3) u32 scale
     sum |q k|, and up to 2^-22 of |q||k| where q is split into two or three terms.  A weight is then off
     by the factor exp(2 e), by ex2's 2^-22 and by its rounding to the product's type; the two sums over n keys
     and the rescalings add n u32 each way.  The output is off by that much of sum w |v|, and by its own
     rounding."""
-    n, hd = k.shape[0], k.shape[2]
-    e = ((hd + 3) * U[F32] + 2.0 ** -22) * abs(scale) * torch.einsum("hd,jhd->hj", x.abs(), k.abs()).amax(1)
+    hd = k.shape[2]
+    n = sees.sum(1)[None]
+    size_qk = torch.einsum("thd,jhd->htj", x.abs(), k.abs()).masked_fill(~sees, 0.0).amax(2)
+    e = ((hd + 3) * U[F32] + 2.0 ** -22) * abs(scale) * size_qk
     rel = torch.expm1(2 * e) + 2.0 ** -20 + 2 * (n + 64) * U[F32] + (2 * U[p_type] if p_type != F32 else 0)
-    size = torch.einsum("hj,jhd->hd", w, v.abs())
-    return rel[:, None] * size + U[out_type] * 1.01 * (size * (1 + rel[:, None])) + 2.0 ** -24
+    rel = rel.transpose(0, 1)[:, :, None]
+    size = torch.einsum("htj,jhd->thd", w, v.abs())
+    return rel * size + U[out_type] * 1.01 * (size * (1 + rel)) + 2.0 ** -24
 
 
 def run_attention(types, heads, hd, page, q_lens, kv_lens, causal=True, window=0, seed=0, junk=math.nan, scale=None,
-                  out=None):
+                  out=None, repeats=0):
     dtype, kv_dtype = types
     hq, hkv = heads
     g = gen(seed + hd + page)
@@ -218,6 +223,9 @@ def run_attention(types, heads, hd, page, q_lens, kv_lens, causal=True, window=0
     kv_len = torch.tensor(kv_lens, dtype=INT, device="cuda")
     got = serving.paged_attention(cache, table, q, q_start, kv_len, max(max(q_lens), 1), scale, causal, window, out)
     want, bound = attention64(cache, table, q, start, lens, hd ** -0.5 if scale is None else scale, causal, window)
+    for _ in range(repeats):
+        assert torch.equal(got, serving.paged_attention(cache, table, q, q_start, kv_len, max(max(q_lens), 1), scale,
+                                                        causal, window))
     serving.attention_check()
     assert got.shape == q.shape and got.dtype == (dtype if out is None else out.dtype)
     err = (got.double() - want).abs()
@@ -290,6 +298,19 @@ def test_attention_long_axis(types, q_len):
 def test_attention_many_sequences(q_lens):
     rng = np.random.RandomState(3)
     run_attention((F16, F16), (4, 1), 64, 16, q_lens, [int(n) + rng.randint(0, 90) for n in q_lens])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,q_lens", [((8, 2), [8]), ((8, 2), [40, 8]), ((8, 2), [64, 5, 32, 9]), ((3, 3), [17]),
+                                          ((3, 3), [130, 17, 256]), ((6, 2), [100, 6, 6])], ids=str)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_many_items_a_cta(dtype, heads, q_lens, hd):
+    """Far more items than CTAs: a CTA runs through items of one tile and of two, whole and in parts, in
+    every order, and does so again."""
+    rng = np.random.RandomState(hd)
+    q = [q_lens[i % len(q_lens)] for i in range(500)]
+    kv = [n + rng.randint(0, 150) for n in q]
+    run_attention((dtype, dtype), heads, hd, 16, q, kv, repeats=30)
 
 
 @pytest.mark.parametrize("types", TYPES, ids=str)
