@@ -23,7 +23,8 @@ namespace {
 
 constexpr int kRows = 16;
 constexpr float kLift = 12.0f;
-constexpr float kJoin = 8.0f;
+// A block's time over that of one row of a part in the CTA that joins it.
+constexpr float kJoin = 64.0f;
 
 DPUF_DEV uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 DPUF_DEV float ex2(float x) {
@@ -93,7 +94,7 @@ paged_attention_rows_kernel(const __grid_constant__ AttnArgs p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hd = p.a.kv.head_dim;
   const AttnParts<kRows, DP> parts(p.a.workspace, gridDim.x);
-  AttnRun run = attn_locate<kRows, kKeys>(p, share, blockIdx.x, gridDim.x, kJoin);
+  AttnRun run = attn_locate<kRows, kKeys>(p, share, blockIdx.x, gridDim.x, kJoin / (float)min(kRows, p.a.max_q * p.group));
   if (run.n == 0) return;
 
   // ---- the warp's stream of keys and values
@@ -353,31 +354,66 @@ paged_attention_rows_kernel(const __grid_constant__ AttnArgs p) {
     }
     if (!whole) {
       const int c0 = attn_cta_of(run, c.begin), c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
-      if (attn_last_part(parts.count + 2 * c0, c1 - c0 + 1, &flag))
+      if (attn_last_part(parts.count + 2 * c0, c1 - c0 + 1, &flag)) {
+        // Of many parts the factors go into shared memory first (where it has room: one long item
+        // among many short ones may be cut into hundreds), so that many loads of outputs are in
+        // flight; of a few, each thread takes them as it goes.
+        const int n = c1 - c0 + 1;
+        float* const fac = merge;  // [rows][n]
+        const bool staged = n > 8 && rows * n <= W * 8 * DP;
+        auto part = [&](int i) { return 2 * (size_t)(c0 + i) + (i == 0); };
+        if (staged) {
+          for (int r = warp; r < rows; r += W) {
+            float top = -CUDART_INF_F;
+            for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(&parts.ml[part(i) * kRows + r]).x);
+            top = warp_max(top);
+            float sum = 0.0f;
+            for (int i = lane; i < n; i += 32) {
+              const float2 ml = __ldcg(&parts.ml[part(i) * kRows + r]);
+              const float g = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
+              fac[r * n + i] = g;
+              sum = __fmaf_rn(ml.y, g, sum);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+            if (lane == 0) ml_sh[0][r].y = sum;
+          }
+          __syncthreads();
+        }
         for (int i = tid; i < rows * (DP / 4); i += W * 32) {
           const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-          float top = -CUDART_INF_F;
-          for (int cc = c0; cc <= c1; cc++)
-            top = fmaxf(top, __ldcg(&parts.ml[(2 * (size_t)cc + (cc == c0)) * kRows + r]).x);
-          float sum = 0.0f;
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int cc = c0; cc <= c1; cc++) {
-            const size_t at = (2 * (size_t)cc + (cc == c0)) * kRows + r;
-            const float2 ml = __ldcg(&parts.ml[at]);
-            const float4 y = __ldcg((const float4*)(parts.o + at * DP + d));
-            const float g = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
-            sum = __fmaf_rn(ml.y, g, sum);
+          float sum = 0.0f;
+          auto add = [&](int k, float g) {
+            const float4 y = __ldcg((const float4*)(parts.o + (part(k) * kRows + r) * DP + d));
             x.x = __fmaf_rn(y.x, g, x.x);
             x.y = __fmaf_rn(y.y, g, x.y);
             x.z = __fmaf_rn(y.z, g, x.z);
             x.w = __fmaf_rn(y.w, g, x.w);
+          };
+          if (staged) {
+            sum = ml_sh[0][r].y;
+#pragma unroll 16
+            for (int k = 0; k < n; k++) add(k, fac[r * n + k]);
+          } else {
+            float top = -CUDART_INF_F;
+#pragma unroll 4
+            for (int k = 0; k < n; k++) top = fmaxf(top, __ldcg(&parts.ml[part(k) * kRows + r]).x);
+#pragma unroll 4
+            for (int k = 0; k < n; k++) {
+              const float2 ml = __ldcg(&parts.ml[part(k) * kRows + r]);
+              const float g = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
+              sum = __fmaf_rn(ml.y, g, sum);
+              add(k, g);
+            }
           }
           const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
-          const int tok = (r0 + r) / p.group, head = c.head * p.group + (r0 + r) % p.group;
+          const int tok = (r0 + r) / p.group, head = c.head * p.group + (r0 + r) - tok * p.group;
           const size_t at = ((size_t)(c.seq.q0 + tok) * p.a.n_q + head) * hd + d;
           if (d < hd) store4_as(p.a.out, at, p.a.out_dtype, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
         }
+        if (staged) __syncthreads();
+      }
     }
     if (left > 0) attn_next_item<kRows, kKeys>(p, c);
   }
