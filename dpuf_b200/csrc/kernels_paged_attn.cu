@@ -187,6 +187,204 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
   }
 }
 
+// ------------------------------------------------------------------ fp32 cache, up to 4 rows
+// Decode steps.  Bound by the bytes of K and V: eight lanes take a key, each some of its dimensions
+// straight into registers (a step ahead), so a warp has four keys at a time and nothing goes
+// through shared memory but the queries; the eight lanes' sums meet in three shuffles a row.  Every
+// group of eight lanes keeps a softmax of its own; they are joined at the item's end.
+constexpr int kFewRows = 4, kFewWarps = 4, kFewKeys = 64;
+constexpr float kFewJoin = 16.0f;
+// CTAs an SM: registers for all that is in flight (64 tokens at 2,304, head_dim 128: 220 us with 2, 305
+// with 3, which spills; 2 tokens at 10,029, head_dim 64: 38 and 36).
+__host__ __device__ constexpr int few_ctas(int dp) { return dp == 64 ? 3 : 2; }
+
+template <int DP>  // head_dim rounded up to 64 or 128
+__global__ void __launch_bounds__(kFewWarps * 32, few_ctas(DP)) paged_attention_f32_few_kernel(const __grid_constant__ AttnArgs p) {
+  constexpr int R = kFewRows, NV = DP / 32, kStep = kFewWarps * 4;  // float4 of a lane, keys of a step
+  __shared__ AttnShare share;
+  __shared__ int flag;
+  __shared__ __align__(16) float qs[R][DP];
+  __shared__ __align__(16) float merge[kFewWarps][R][DP];
+  __shared__ float2 ml_sh[kFewWarps][R];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 3, gl = lane & 7;
+  const int hd = p.a.kv.head_dim;
+  AttnRun run = attn_locate<R, kFewKeys>(p, share, blockIdx.x, gridDim.x, kFewJoin);
+  if (run.n == 0) return;
+  const AttnParts<R, DP> parts(p.a.workspace, gridDim.x);
+  AttnCursor& c = run.cur;
+
+  for (int left = run.n; left > 0;) {
+    const int from = c.at, to = min(c.n_blk, c.at + left);
+    left -= to - from;
+    const int total = c.seq.qn * p.group, r0 = c.tile * R, rows = min(R, total - r0);
+    __syncthreads();
+    for (int i = tid; i < R * DP; i += kFewWarps * 32) {
+      const int r = i / DP, d = i % DP, tok = (r0 + r) / p.group;
+      qs[r][d] = r < rows && d < hd ? load_as(p.a.q, (size_t)((int64_t)(c.seq.q0 + tok) * p.a.q_stride[0] +
+                                              (int64_t)(c.head * p.group + r0 + r - tok * p.group) * p.a.q_stride[1] + d),
+                                              p.a.dtype) * (p.a.scale * kLog2e)
+                                    : 0.0f;
+    }
+    int lo[R], hi[R];  // positions that each row sees
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      lo[r] = hi[r] = 0;
+      if (r < rows) attn_span(p, c.seq, (r0 + r) / p.group, (r0 + r) / p.group, &lo[r], &hi[r]);
+    }
+    int tlo, thi;  // positions that the tile sees
+    attn_span(p, c.seq, r0 / p.group, min(c.seq.qn - 1, (r0 + R - 1) / p.group), &tlo, &thi);
+    __syncthreads();
+    float m[R], l[R], o[R][NV * 4];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      m[r] = -CUDART_INF_F;
+      l[r] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < NV * 4; e++) o[r][e] = 0.0f;
+    }
+    const int first = (c.blk0 + from) * kFewKeys + warp * 4 + grp, steps = (to - from) * (kFewKeys / kStep);
+    auto page_of = [&](int step) -> int64_t {
+      const int j = first + step * kStep;
+      return step < steps && j >= tlo && j < thi ? attn_page(p, c.s, j) : -1;
+    };
+    float4 k[NV], v[NV];
+    auto fetch = [&](int step, int64_t page, float4 (&kk)[NV], float4 (&vv)[NV]) {
+      const int j = first + step * kStep;
+      const int64_t at = page + (int64_t)c.head * p.a.kv.head_stride +
+                         (int64_t)(j & (p.a.kv.page_size - 1)) * p.a.kv.row_stride + gl * 4;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        kk[i] = vv[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (page >= 0 && i * 32 + gl * 4 < hd) {
+          kk[i] = __ldcs((const float4*)((const float*)p.a.kv.k + at + i * 32));
+          vv[i] = __ldcs((const float4*)((const float*)p.a.kv.v + at + i * 32));
+        }
+      }
+    };
+    int64_t page = page_of(0);
+    fetch(0, page, k, v);
+    page = page_of(1);
+    for (int step = 0; step < steps; step++) {
+      float4 k2[NV], v2[NV];
+      fetch(step + 1, page, k2, v2);
+      page = page_of(step + 2);
+      const int j = first + step * kStep;
+      float s[R], f[R];
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        s[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+          const float4 q = *(const float4*)&qs[r][i * 32 + gl * 4];
+          s[r] = fmaf(q.x, k[i].x, fmaf(q.y, k[i].y, fmaf(q.z, k[i].z, fmaf(q.w, k[i].w, s[r]))));
+        }
+      }
+      bool grew = false;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+#pragma unroll
+        for (int i = 1; i < 8; i <<= 1) s[r] += __shfl_xor_sync(kFull, s[r], i);
+        if (!(j >= lo[r] && j < hi[r])) s[r] = -CUDART_INF_F;
+        const float m2 = fmaxf(m[r], s[r]);
+        f[r] = m2 == m[r] ? 1.0f : ex2(m[r] - m2);
+        s[r] = s[r] == -CUDART_INF_F ? 0.0f : ex2(s[r] - m2);
+        grew = grew || f[r] != 1.0f;
+        l[r] = fmaf(l[r], f[r], s[r]);
+        m[r] = m2;
+      }
+      if (__any_sync(kFull, grew))
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+          for (int e = 0; e < NV * 4; e++) o[r][e] *= f[r];
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+          o[r][4 * i] = fmaf(s[r], v[i].x, o[r][4 * i]);
+          o[r][4 * i + 1] = fmaf(s[r], v[i].y, o[r][4 * i + 1]);
+          o[r][4 * i + 2] = fmaf(s[r], v[i].z, o[r][4 * i + 2]);
+          o[r][4 * i + 3] = fmaf(s[r], v[i].w, o[r][4 * i + 3]);
+        }
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        k[i] = k2[i];
+        v[i] = v2[i];
+      }
+    }
+    // ---- the warp's four groups, then the warps
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+#pragma unroll
+      for (int x = 8; x < 32; x <<= 1) {
+        const float om = __shfl_xor_sync(kFull, m[r], x), ol = __shfl_xor_sync(kFull, l[r], x);
+        const float m2 = fmaxf(m[r], om);
+        const float g = m[r] == -CUDART_INF_F ? 0.0f : ex2(m[r] - m2), og = om == -CUDART_INF_F ? 0.0f : ex2(om - m2);
+        l[r] = l[r] * g + ol * og;
+        m[r] = m2;
+#pragma unroll
+        for (int e = 0; e < NV * 4; e++) {
+          const float y = __shfl_xor_sync(kFull, o[r][e], x);
+          o[r][e] = o[r][e] * g + y * og;
+        }
+      }
+      if (grp == 0)
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+          *(float4*)&merge[warp][r][i * 32 + gl * 4] =
+              make_float4(o[r][4 * i], o[r][4 * i + 1], o[r][4 * i + 2], o[r][4 * i + 3]);
+      if (lane == 0) ml_sh[warp][r] = make_float2(m[r], l[r]);
+    }
+    __syncthreads();
+    const bool whole = from == 0 && to == c.n_blk;
+    const int r = tid / (DP / 4), d = tid % (DP / 4) * 4;  // one float4 of the tile's output a thread
+    const bool mine = r < rows;
+    float top = -CUDART_INF_F, sum = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](float2 ml, float4 y) {
+      const float g = ml.x == -CUDART_INF_F ? 0.0f : ex2(ml.x - top);
+      sum = fmaf(ml.y, g, sum);
+      x.x = fmaf(y.x, g, x.x);
+      x.y = fmaf(y.y, g, x.y);
+      x.z = fmaf(y.z, g, x.z);
+      x.w = fmaf(y.w, g, x.w);
+    };
+    if (mine) {
+#pragma unroll
+      for (int w = 0; w < kFewWarps; w++) top = fmaxf(top, ml_sh[w][r].x);
+#pragma unroll
+      for (int w = 0; w < kFewWarps; w++) add(ml_sh[w][r], *(const float4*)&merge[w][r][d]);
+    }
+    bool join = false;
+    if (!whole) {
+      const size_t slot = 2 * (size_t)blockIdx.x + (from == 0 ? 1 : 0);
+      if (mine) {
+        if (d == 0) parts.ml[slot * R + r] = make_float2(top, sum);
+        *(float4*)(parts.o + (slot * R + r) * DP + d) = x;
+      }
+      const int c0 = attn_cta_of(run, c.begin), c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
+      join = attn_last_part(parts.count + 2 * c0, c1 - c0 + 1, &flag);
+      if (join && mine) {
+        top = -CUDART_INF_F;
+        sum = 0.0f;
+        x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto at = [&](int cc) { return (2 * (size_t)cc + (cc == c0)) * R + r; };
+#pragma unroll 8
+        for (int cc = c0; cc <= c1; cc++) top = fmaxf(top, __ldcg(&parts.ml[at(cc)]).x);
+#pragma unroll 8
+        for (int cc = c0; cc <= c1; cc++) add(__ldcg(&parts.ml[at(cc)]), __ldcg((const float4*)(parts.o + at(cc) * DP + d)));
+      }
+    }
+    if ((whole || join) && mine && d < hd) {
+      const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
+      const int tok = (r0 + r) / p.group, head = c.head * p.group + r0 + r - tok * p.group;
+      store4_as(p.a.out, ((size_t)(c.seq.q0 + tok) * p.a.n_q + head) * hd + d, p.a.out_dtype, x.x * inv, x.y * inv,
+                x.z * inv, x.w * inv);
+    }
+    if (left > 0) attn_next_item<R, kFewKeys>(p, c);
+  }
+}
+
 template <typename TK, int DP>
 cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
   constexpr size_t smem = sizeof(float) * (kGenRows * DP + 2 * kGenKeys * (DP + 4) + kGenRows * (kGenKeys + 1));
@@ -199,7 +397,9 @@ cudaError_t launch_f32(const AttnArgs& p, cudaStream_t s) {
 }  // namespace
 
 int64_t paged_attention_workspace() {
-  return (int64_t)std::max(AttnParts<kGenRows, 256>::bytes(kAttnSms * 2), paged_attention_tc_workspace());
+  static_assert(kAttnSms * 3 <= kAttnMaxCtas, "counters");
+  return (int64_t)std::max({AttnParts<kGenRows, 256>::bytes(kAttnSms * 2), AttnParts<kFewRows, 128>::bytes(kAttnSms * 3),
+                            paged_attention_tc_workspace()});
 }
 
 cudaError_t paged_attention_status(void* workspace, bool* gave_up, cudaStream_t s) {
@@ -218,6 +418,14 @@ cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t
   p.page_shift = 31 - __builtin_clz((unsigned)a.kv.page_size);
   p.max_kv = (int)std::min<int64_t>((int64_t)a.pages_per_seq << p.page_shift, 1 << 30);
   if (a.kv.dtype == DPUF_TYPE_F32) {
+    // up to 4 rows stream (64 tokens at 2,304, 32 / 8 heads of 128: 220 us; by the 16-row tiles 680)
+    if (a.max_q * p.group <= kFewRows && a.kv.head_dim <= 128) {
+      if (a.kv.head_dim <= 64)
+        paged_attention_f32_few_kernel<64><<<kAttnSms * few_ctas(64), kFewWarps * 32, 0, s>>>(p);
+      else
+        paged_attention_f32_few_kernel<128><<<kAttnSms * few_ctas(128), kFewWarps * 32, 0, s>>>(p);
+      return cudaGetLastError();
+    }
     if (a.kv.head_dim <= 64) return launch_f32<float, 64>(p, s);
     if (a.kv.head_dim <= 128) return launch_f32<float, 128>(p, s);
     return launch_f32<float, 256>(p, s);
