@@ -59,7 +59,8 @@ cudaError_t smem_limit_once(int bytes) {
   return e;
 }
 
-// 16-bit queries and cache, head_dim <= 128 (kernels_paged_attn_tc.cu).
+// 16-bit queries and cache, head_dim <= 128 (kernels_paged_attn_tc.cu); cudaErrorNotSupported where
+// no tensor map holds the cache's strides.
 cudaError_t launch_paged_attention_tc(const AttnArgs& p, cudaStream_t s);
 size_t paged_attention_tc_workspace();
 // 16-bit cache, queries of its type or (head_dim <= 128) fp32 (kernels_paged_attn_rows.cu).

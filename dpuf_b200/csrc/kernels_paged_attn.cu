@@ -432,7 +432,12 @@ cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t
   }
   if (a.dtype == DPUF_TYPE_F32 && a.kv.head_dim > 128)
     return a.kv.dtype == DPUF_TYPE_F16 ? launch_f32<__half, 256>(p, s) : launch_f32<__nv_bfloat16, 256>(p, s);
-  if (a.dtype != DPUF_TYPE_F32 && a.kv.head_dim <= 128 && a.max_q * p.group > 16) return launch_paged_attention_tc(p, s);
+  // more rows than one mma.sync tile: 32 sequences of 2,000 positions with 32 / 64 rows each take the
+  // tensor-core kernel 87 / 87 us, the streaming one 105 / 186; one of 16 rows at 2,304 17 us there
+  if (a.dtype != DPUF_TYPE_F32 && a.kv.head_dim <= 128 && a.max_q * p.group > 16) {
+    const cudaError_t e = launch_paged_attention_tc(p, s);
+    if (e != cudaErrorNotSupported) return e;  // (a cache whose strides no tensor map holds streams)
+  }
   return launch_paged_attention_rows(p, s);
 }
 

@@ -829,7 +829,7 @@ cudaError_t launch_paged_attention_tc(const AttnArgs& p, cudaStream_t s) {
   const cuuint64_t strides[3] = {(cuuint64_t)kv.row_stride, (cuuint64_t)kv.head_stride, (cuuint64_t)kv.page_stride};
   const cuuint32_t box[4] = {64, (cuuint32_t)std::min(kv.page_size, kKeys), 1, 1};
   if (!encode(&a.k_map, kv.dtype, kv.k, 4, dims, strides, box) || !encode(&a.v_map, kv.dtype, kv.v, 4, dims, strides, box))
-    return cudaErrorInvalidValue;
+    return cudaErrorNotSupported;  // strides that a tensor map cannot hold
   const cuuint64_t q_dims[3] = {(cuuint64_t)kv.head_dim, (cuuint64_t)p.a.n_q, (cuuint64_t)p.a.n_tokens};
   const cuuint64_t q_strides[2] = {(cuuint64_t)p.a.q_stride[1], (cuuint64_t)p.a.q_stride[0]};
   const cuuint32_t q_box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(kTile / p.group)};

@@ -109,7 +109,7 @@ struct SampleShared {
   u64 warp_sum[kSampWarps];
   float warp_lo[kSampWarps], warp_hi[kSampWarps];
   Found found;
-  int step_k, step_p;
+  int step_k, step_p, step_lo;
   float hi_k, hi_m;
 };
 
@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
   bool by_k = false, by_p = false;  // filters that may end the prefix
   u64 mass = 0;                     // weight of what top-k keeps, where by_p
   int last_step = kBins;            // kBins: the whole slice stays the domain
+  int first_step = 0;               // top-p ends no earlier
   if (limit_k || limit_p) {
     auto whole_mass = [&]() {
       u64 mine = 0;
@@ -340,7 +341,10 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
       sh.warp_lo[tid >> 5] = sl;
       sh.warp_hi[tid >> 5] = sh_;
     }
-    if (tid == 0) sh.step_k = sh.step_p = kBins;
+    if (tid == 0) {
+      sh.step_k = sh.step_p = kBins;
+      sh.step_lo = 0;
+    }
     __syncthreads();
     float all_lo = 0.0f;
 #pragma unroll
@@ -379,7 +383,13 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
 #pragma unroll
       for (int e = 0; e < 2; e++)
         if (run_lo[e] >= target && (2 * tid + e == 0 || run_lo[e] - lo[e] < target)) atomicMin(&sh.step_p, 2 * tid + e);
+      // and the last step before which it has not ended for sure
+      const float least = top_p * (float)((double)mass / (double)kFix) * 0.999f;
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        if (!by_k && run_hi[e] < least) atomicMax(&sh.step_lo, 2 * tid + e + 1);
       __syncthreads();
+      first_step = min(sh.step_lo, kBins - 1);
     }
     // top-p after a top-k that ends the prefix needs all that top-k keeps for its weight
     last_step = by_k ? sh.step_k : sh.step_p;
@@ -545,10 +555,11 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
   };
   // Entries with keys in [lo, hi] into bins of 2^shift keys from the top, and the bin in which the
   // count (by_count) or the weight, from the sums above, reaches the target.
+  // `tail`: the range is all that lies below its top, so what lies above is the rest of the whole.
   // (top-p's first range is top-k's: its histogram is kept where top-k needed no other.)
   uint32_t built_lo = 1, built_hi = 0;
-  auto level = [&](uint32_t lo, uint32_t hi, int shift, bool by_count, const Found above, uint32_t k_target,
-                   double p_target) {
+  auto level = [&](uint32_t lo, uint32_t hi, int shift, bool by_count, Found above, uint32_t k_target,
+                   double p_target, bool tail) {
     const bool again = lo == built_lo && hi == built_hi;
     built_lo = lo;
     built_hi = hi;
@@ -636,6 +647,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
     }
     if (tid < 32) {
       const u64 c0 = lane < R ? of(lane)->seg_count : 0, f0 = lane < R ? of(lane)->seg_mass : 0;
+      if (tail) above.mass_above = mass - __shfl_sync(kFull, warp_inclusive(f0), 31);
       const u64 ci = warp_inclusive(c0) + above.above, fi = warp_inclusive(f0) + above.mass_above;
       const unsigned in = __ballot_sync(kFull, lane < R && c0 > 0 && reached(by_count, ci, fi, k_target, p_target));
       if (in) {
@@ -662,12 +674,26 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
   // the value in which the target is reached: its key, the sums above it and its own (bin -1: not
   // reached in the domain)
   auto select = [&](bool by_count, uint32_t k_target, double p_target, uint32_t* key) {
-    uint32_t hi = key_max, lo = max(1u, Key<T>::of(cut));
+    // down to the domain's end, or to where weights end
+    const float end = m - reach * temp, slack = 1e-5f * (fabsf(m) + fabsf(end)) + 1e-30f;
+    const float all = end - slack == end - slack ? end - slack : -CUDART_INF_F;
+    uint32_t hi = key_max, lo = max(1u, Key<T>::of(fmaxf(cut, all)));
+    // over all slices, of a top-p alone: from the step before which it has not ended, down to the
+    // smallest weight, so that what is above follows from the whole
+    bool tail = false;
+    if (!by_count && !by_k && !local && first_step > 0) {
+      const float high = m - (float)first_step / per_step * temp + slack;
+      if (high >= all && high < m) {
+        lo = max(1u, Key<T>::of(all));
+        hi = Key<T>::of(high);
+        tail = true;
+      }
+    }
     Found f{0, 0, 0, 0, 0};
-    for (;;) {
+    for (;; tail = false) {
       int shift = 0;
       while (((hi - lo) >> shift) >= (uint32_t)kBins) shift++;
-      f = level(lo, hi, shift, by_count, f, k_target, p_target);
+      f = level(lo, hi, shift, by_count, f, k_target, p_target, tail);
       if (f.bin < 0) return f;
       const uint32_t top = hi - ((uint32_t)f.bin << shift);
       if (shift == 0) {

@@ -270,6 +270,25 @@ def test_attention_window(types, window):
 
 
 @pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("q_len,hd", [(1, 64), (1, 128), (6, 64), (200, 128)])
+def test_attention_places_before_the_window(types, q_len, hd):
+    """Positions in held pages that lie before every window may hold anything."""
+    g = gen(31)
+    dtype, kv_dtype = types
+    table, n_pages = table_for([700], 64, g)
+    k, v = (normal(g, n_pages, 2, 64, hd, dtype=kv_dtype) for _ in range(2))
+    at = torch.arange(700 - q_len - 99, device="cuda")  # the first token sees 100 positions
+    k[table[0, at // 64].long(), :, at % 64] = math.nan
+    v[table[0, at // 64].long(), :, at % 64] = math.inf
+    cache = serving.PagedCache(k, v)
+    q = normal(g, q_len, 4, hd, dtype=dtype)
+    got = serving.paged_attention(cache, table, q, torch.tensor([0, q_len], dtype=INT, device="cuda"),
+                                  torch.tensor([700], dtype=INT, device="cuda"), q_len, window=100)
+    want, bound = attention64(cache, table, q, [0, q_len], [700], hd ** -0.5, True, 100)
+    assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
 @pytest.mark.parametrize("q_lens", [[1, 1, 0, 1], [5, 3, 0, 200]], ids=str)
 def test_attention_empty_rows(types, q_lens):
     """Sequences without positions, tokens before the first position, sequences without tokens."""
@@ -578,6 +597,32 @@ def test_sample_ties_go_to_the_lowest_index(dtype, vocab):
     ids, probs = serving.sample(same, torch.tensor(u, device="cuda"), None,
                                 torch.full((rows,), 64, dtype=INT, device="cuda"))
     assert ids.tolist() == [int(x * 64) for x in u] and bool((probs == 1 / 64).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("spread", [0.01, 0.3, 1.0, 2.0])
+def test_sample_large_nuclei(dtype, spread):
+    """Flat rows: a nucleus of much of the vocabulary, which no CTA can be handed."""
+    rng = np.random.RandomState(int(100 * spread))
+    for vocab in (3001, 90000, 151936):
+        logits = (torch.from_numpy(rng.standard_normal((8, vocab)).astype(np.float32)) * spread).to(dtype).cuda()
+        u = rng.random_sample(8).astype(np.float32)
+        temp = rng.choice([0.5, 1.0, 1.5], 8).astype(np.float32)
+        for p in (0.5, 0.9, 0.99, 0.9999):
+            check_rows(logits, u, temp, None, [p] * 8)
+        check_rows(logits, u, temp, [vocab // 2] * 8, [0.97] * 8)
+        check_rows(logits, u, temp, None, [0.97] * 8, [0.05] * 8)
+
+
+def test_sample_rows_beyond_shared_memory():
+    """The longest rows do not fit the cluster's shared memory: what does not is read again."""
+    rng = np.random.RandomState(4)
+    logits = (torch.from_numpy(rng.standard_normal((3, 1 << 20)).astype(np.float32)) * 2).cuda()
+    u = rng.random_sample(3).astype(np.float32)
+    check_rows(logits, u)
+    check_rows(logits, u, None, [40] * 3, [0.9] * 3)
+    check_rows(logits, u, None, None, [0.95] * 3)
+    check_rows(logits[:, 1:], u, None, [100000] * 3, [0.99] * 3)
 
 
 def test_sample_unusual_values():
