@@ -12,6 +12,8 @@
 // An item counts kLead blocks more than it has, for what it costs beside them (queries, results,
 // the pipeline's filling): they stand before its first, and a run that ends in them leaves the
 // whole item to the next.
+// A cut within kSnap places of an item's end moves there: joining parts costs more than the two
+// CTAs' work then differs by.
 //   part of an item that began in an earlier CTA: slot 2c; part that a later CTA goes on with:
 //   slot 2c + 1; the counter is that of the CTA in which the item begins.
 #pragma once
@@ -72,11 +74,20 @@ struct AttnCursor {
   long long begin;    // the item's first block in the sequence of all
 };
 
+// Of an item of n blocks: cuts up to *lo places in move to its start, those from *hi on to its end.
+template <int kLead, int kSnap>
+DPUF_DEV void attn_snap(int n, int* lo, int* hi) {
+  *lo = max(min(kSnap, (n + kLead) / 2), kLead);
+  *hi = max(n + kLead - min(kSnap, (n + kLead - 1) / 2), *lo + 1);
+}
+
 // The blocks [*from, *to) of the cursor's item that a run with `left` places takes, maybe none.
-template <int kLead>
+template <int kLead, int kSnap = 0>
 DPUF_DEV void attn_take(const AttnCursor& c, int& left, int* from, int* to) {
-  const int end = min(c.n_blk + kLead, c.at + left);
-  left -= end - c.at;
+  int end = c.at + left, lo, hi;
+  attn_snap<kLead, kSnap>(c.n_blk, &lo, &hi);
+  left = max(end - (c.n_blk + kLead), 0);
+  end = end <= lo ? c.at : end >= hi ? c.n_blk + kLead : end;
   *from = max(c.at - kLead, 0);
   *to = max(end - kLead, 0);
 }
@@ -166,7 +177,7 @@ DPUF_DEV long long attn_scan(long long v) {  // inclusive, over the warp
 //
 // All threads of the CTA call this together.  A warp adds up a run of sequences, 32 at a time; the
 // warp in whose run the CTA's first block lies finds it.
-template <int BM, int BN, int kLead = 0>
+template <int BM, int BN, int kLead = 0, int kSnap = 0>
 DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas, float join) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   const int per = (p.a.n_seqs + nw - 1) / nw;
@@ -241,11 +252,27 @@ DPUF_DEV AttnRun attn_locate(const AttnArgs& p, AttnShare& sh, int cta, int ctas
   }
   __syncthreads();
   r.cur = sh.start;
+  int lo, hi;
+  attn_snap<kLead, kSnap>(r.cur.n_blk, &lo, &hi);
+  if (r.cur.at <= lo) {
+    r.n += r.cur.at;
+    r.cur.at = 0;
+  } else if (r.cur.at >= hi) {
+    r.n = max(r.n - (r.cur.n_blk + kLead - r.cur.at), 0);
+    if (r.n) attn_next_item<BM, BN, kLead>(p, r.cur);
+  }
   return r;
 }
 
-// The CTA that holds place x of all.
-DPUF_DEV int attn_cta_of(const AttnRun& r, long long x) { return (int)(((x + 1) * r.ctas - 1) / r.total); }
+// The first and last CTA that have parts of the cursor's item.
+template <int kLead = 0, int kSnap = 0>
+DPUF_DEV void attn_owners(const AttnRun& r, const AttnCursor& c, int* c0, int* c1) {
+  int lo, hi;
+  attn_snap<kLead, kSnap>(c.n_blk, &lo, &hi);
+  auto holds = [&](long long x) { return (int)(((x + 1) * r.ctas - 1) / r.total); };  // place x of all
+  *c0 = holds(c.begin + lo);
+  *c1 = holds(c.begin + hi - 1);
+}
 
 // Cache offset (elements) of head 0, row 0 of the page that holds position j of sequence s, or -1.
 DPUF_DEV int64_t attn_page(const AttnArgs& p, int s, int j) {

@@ -25,7 +25,8 @@ DPUF_DEV float ex2(float x) {
 }
 
 // ------------------------------------------------------------------ fp32 arithmetic, any types
-// A CTA takes 16 rows and blocks of 32 keys, both widened to fp32 in shared memory.  Thread
+// Chunks over an fp32 cache, and fp32 queries of heads over 128.  Bound by shared-memory reads (a
+// float4 of K or V feeds 4 or 8 multiply-adds).  A CTA takes 16 rows and blocks of 32 keys, both widened to fp32 in shared memory.  Thread
 // (row = tid / 16, x = tid % 16) has the scores of keys x and x + 16 and the output's dimensions
 // 4 x + 64 i of its row; a row's 16 threads are half a warp.
 constexpr int kGenRows = 16, kGenKeys = 32, kGenThreads = 256;
@@ -145,8 +146,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
       for (int i = 0; i < DP / 64; i++)
         *(float4*)(parts.o + (slot * kGenRows + row) * DP + 64 * i + 4 * x) =
             make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-      c0 = attn_cta_of(run, c.begin);
-      c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
+      attn_owners(run, c, &c0, &c1);
       join = attn_last_part(parts.count + 2 * c0, c1 - c0 + 1, &flag);
       if (join) {
         m = -CUDART_INF_F;
@@ -362,7 +362,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_ctas(DP)) paged_attention_
         if (d == 0) parts.ml[slot * R + r] = make_float2(top, sum);
         *(float4*)(parts.o + (slot * R + r) * DP + d) = x;
       }
-      const int c0 = attn_cta_of(run, c.begin), c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
+      int c0, c1;
+      attn_owners(run, c, &c0, &c1);
       join = attn_last_part(parts.count + 2 * c0, c1 - c0 + 1, &flag);
       if (join && mine) {
         top = -CUDART_INF_F;

@@ -353,7 +353,8 @@ paged_attention_rows_kernel(const __grid_constant__ AttnArgs p) {
       __syncthreads();
     }
     if (!whole) {
-      const int c0 = attn_cta_of(run, c.begin), c1 = attn_cta_of(run, c.begin + c.n_blk - 1);
+      int c0, c1;
+      attn_owners(run, c, &c0, &c1);
       if (attn_last_part(parts.count + 2 * c0, c1 - c0 + 1, &flag)) {
         // Of many parts the factors go into shared memory first (where it has room: one long item
         // among many short ones may be cut into hundreds), so that many loads of outputs are in

@@ -49,6 +49,11 @@ constexpr int kLoadWarp = 8, kMmaWarp = 9, kQueryWarp = 11;  // kMmaWarp + i: ti
 constexpr int kThreads = 384;
 // What an item costs beside its blocks, in blocks (four prompts of 2,048: 178 us at 0, 167 at 2, 168 at 3, 174 at 5).
 constexpr int kLead = 2;
+// Cuts that move to an item's end (a part of 256 rows is 128 KB out and in again).  49 x 216 tokens
+// of 3 heads: 31 us at 0, 20 at 3, 19 at 6 and 12; four prompts of 2,048: 170, 167, 167, 170.
+constexpr int kSnap = 6;
+// Few items are cut into fewer parts (attn_locate).  One prompt of 1,000 tokens, 32/8 heads: 45 us,
+// 52 at 0.1, 46 without a limit; 64 tokens over 20,000, 8/2 heads: 67 us, 89 at 0.1, 150 without.
 constexpr float kJoin = 0.33f;
 // The weights carry a factor 2^7, and so does their sum: at most 2^15, which fp16 holds, while the
 // small ones of a long context keep their bits.
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     abort_sh = 0;
   }
   fence_before();
-  AttnRun run = attn_locate<kItemRows, kKeys, kLead>(p, share, blockIdx.x, gridDim.x, kJoin);
+  AttnRun run = attn_locate<kItemRows, kKeys, kLead, kSnap>(p, share, blockIdx.x, gridDim.x, kJoin);
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_sh;
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     for (int left = run.n; ok && left > 0;) {
       int from, to, lo, hi;
       const int done = run.n - left;
-      attn_take<kLead>(c, left, &from, &to);
+      attn_take<kLead, kSnap>(c, left, &from, &to);
       const int n = to - from;
       const AttnOrder order(c, from, n, done, length);
       item_span(p, c.seq, c.tile, &lo, &hi);
@@ -356,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     for (int left = run.n; ok && left > 0;) {
       const unsigned seg = asked;
       int from, to;
-      attn_take<kLead>(c, left, &from, &to);
+      attn_take<kLead, kSnap>(c, left, &from, &to);
       if (from == to) {
         if (left > 0) attn_next_item<kItemRows, kKeys, kLead>(p, c);
         continue;
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     for (int left = run.n; ok && left > 0;) {
       int from, to, lo, hi;
       const int done = run.n - left;
-      attn_take<kLead>(c, left, &from, &to);
+      attn_take<kLead, kSnap>(c, left, &from, &to);
       const int n = to - from;
       const AttnOrder order(c, from, n, done, length);
       if (n == 0) {
@@ -525,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     for (int left = run.n; ok && left > 0;) {
       int from, to;
       const int done = run.n - left;
-      attn_take<kLead>(c, left, &from, &to);
+      attn_take<kLead, kSnap>(c, left, &from, &to);
       const int n = to - from;
       const AttnOrder order(c, from, n, done, length);
       if (n == 0) {
@@ -631,8 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
           for (int e = 0; e < 32; e++)  // [dim][row]: a warp's rows are adjacent
             parts.o[(slot * DP + 32 * i + e) * kItemRows + pr] = __uint_as_float(o[e]);
         }
-        c0 = attn_cta_of(run, c.begin + kLead);
-        c1 = attn_cta_of(run, c.begin + kLead + c.n_blk - 1);
+        attn_owners<kLead, kSnap>(run, c, &c0, &c1);
         __threadfence();
         wg_sync();
         if (t == 0) flag_sh[w] = attn_arrive(parts.count + 2 * c0 + w, c1 - c0 + 1);

@@ -332,6 +332,14 @@ def test_attention_many_items_a_cta(dtype, heads, q_lens, hd):
     run_attention((dtype, dtype), heads, hd, 16, q, kv, repeats=30)
 
 
+@pytest.mark.parametrize("heads,seqs,q_len,kv_len", [((3, 3), 49, 216, 216), ((3, 3), 58, 216, 300), ((4, 2), 20, 70, 900),
+                                                      ((4, 1), 37, 100, 1100), ((2, 2), 41, 257, 777), ((8, 2), 1, 333, 2500)])
+def test_attention_cuts_at_item_ends(heads, seqs, q_len, kv_len):
+    """Items from a few key blocks to some forty, so that the cuts between CTAs fall at every distance from
+    an item's ends: moved there, or left where they are with several in one item."""
+    run_attention((F16, F16), heads, 64, 32, [q_len] * seqs, [kv_len - 3 * i % q_len for i in range(seqs)], repeats=3)
+
+
 @pytest.mark.parametrize("types", TYPES, ids=str)
 def test_attention_scale_and_out(types):
     out = torch.empty(9, 4, 64, dtype=F32, device="cuda")
