@@ -154,6 +154,24 @@ DPUF_DEV u64 block_sum(u64 v, u64* warp_sum) {
   return v;
 }
 
+// Bit j: entry j of 16 bytes is `cut` or more (NaN is not).
+DPUF_DEV uint32_t at_least(uint4 x, float cut, float) {
+  return (uint32_t)(__uint_as_float(x.x) >= cut) | (uint32_t)(__uint_as_float(x.y) >= cut) << 1 |
+         (uint32_t)(__uint_as_float(x.z) >= cut) << 2 | (uint32_t)(__uint_as_float(x.w) >= cut) << 3;
+}
+DPUF_DEV uint32_t at_least_bits(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // from two 16-bit masks each
+  const uint32_t t = (a & 0x00010001u) | (b & 0x00010001u) << 2 | (c & 0x00010001u) << 4 | (d & 0x00010001u) << 6;
+  return (t | t >> 15) & 0xFFu;
+}
+DPUF_DEV uint32_t at_least(uint4 x, float cut, __half) {
+  const __half2 c = __half2half2(__float2half_ru(cut)), *e = (const __half2*)&x;
+  return at_least_bits(__hge2_mask(e[0], c), __hge2_mask(e[1], c), __hge2_mask(e[2], c), __hge2_mask(e[3], c));
+}
+DPUF_DEV uint32_t at_least(uint4 x, float cut, __nv_bfloat16) {
+  const __nv_bfloat162 c = __bfloat162bfloat162(__float2bfloat16_ru(cut)), *e = (const __nv_bfloat162*)&x;
+  return at_least_bits(__hge2_mask(e[0], c), __hge2_mask(e[1], c), __hge2_mask(e[2], c), __hge2_mask(e[3], c));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -270,11 +288,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
   // steps per unit of (m - l) / T; a little more than the row's span, so that its smallest entry is inside
   const float span = (m - low_v) * inv_t * 1.0001f + 1e-6f;
   const float reach = span < kReach ? span : kReach;  // (kReach for an infinite or undefined span)
-  const float per_step = (float)kBins / reach;
-  auto step_of = [&](float v) {  // -1: beyond the reach, or NaN
-    const float z = v == m ? 0.0f : (m - v) * inv_t;
-    return z < reach ? min((int)(z * per_step), kBins - 1) : -1;
-  };
+  const float per_step = (float)kBins / reach, per_unit = inv_t * per_step;
   // every entry of the slice, in no order: 16 bytes at a time
   auto each = [&](auto f) {
     const int full = min(n, a.cached) / kVec * kVec;
@@ -304,10 +318,16 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
       mine = block_sum(mine, sh.warp_sum);
       if (tid == 0) sh.exchange[0] = mine;
     };
-    each([&](float v) {
-      const int b = step_of(v);
-      if (b >= 0) atomicAdd(&sh.count[b], 1u);
-    });
+    if (m < CUDART_INF_F && per_unit < CUDART_INF_F)
+      each([&](float v) {
+        const float z = (m - v) * per_unit;
+        if (z < (float)kBins) atomicAdd(&sh.count[(int)z], 1u);  // (not for NaN)
+      });
+    else  // m - m may be no number, and the steps' factor no finite one
+      each([&](float v) {
+        const float z = v == m ? 0.0f : (m - v) * inv_t;
+        if (z < reach) atomicAdd(&sh.count[min((int)(z * per_step), kBins - 1)], 1u);
+      });
     const bool mass_now = limit_p && !limit_k && !(min_p > 0.0f);  // else it may not be needed
     if (mass_now) whole_mass();
     cl.sync();
@@ -397,7 +417,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
   }
 
   // ---- 3. the entries down to that step to rank 0: at once while they are few, else once its
-  // slice is free.  In index order: a warp has a run of the slice, a lane 16 bytes of each step.
+  // slice is free.  In index order: a thread's run is contiguous.
   float cut = -CUDART_INF_F;
   bool local = false;  // rank 0 goes on alone, over what it has been given
   int have = 0;
@@ -407,68 +427,54 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
     const float low = m - (float)(last_step + 1) / per_step * temp;
     cut = fminf(low - 1e-5f * (fabsf(m) + fabsf(low)) - 1e-30f, m);  // at or below every entry wanted
     if (!(cut <= m)) cut = -CUDART_INF_F;                             // the step's end is not finite
-    constexpr int kStep = 32 * kVec;
-    const int steps = (n + kStep - 1) / kStep, warp = tid >> 5;
-    const int s0 = steps * warp / kSampWarps, s1 = steps * (warp + 1) / kSampWarps;
-    auto lane_values = [&](int s, float (&v)[kVec]) {  // NaN beyond the slice
-      const int i = s * kStep + lane * kVec;
-      if (i + kVec <= min(n, a.cached)) {
-        const uint4 x = *(const uint4*)(cache + i);
-        const T* e = (const T*)&x;
+    // runs of an odd number of 16 bytes (no bank conflicts), eight at a time, as bits
+    const int vectors_ = (n + kVec - 1) / kVec, per = ((vectors_ + kSampThreads - 1) / kSampThreads) | 1;
+    const int v0 = min(tid * per, vectors_), v1 = min(v0 + per, vectors_);
+    typedef typename std::conditional<kVec == 8, u64, uint32_t>::type Bits;
+    auto wanted = [&](int first) {
+      Bits in = 0;
 #pragma unroll
-        for (int j = 0; j < kVec; j++) v[j] = to_f32(e[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; j++) v[j] = i + j < n ? at(i + j) : CUDART_NAN_F;
+      for (int x = 0; x < 8; x++) {
+        const int i = (first + x) * kVec;
+        if (first + x >= v1) break;
+        if (i + kVec <= min(n, a.cached))
+          in |= (Bits)at_least(*(const uint4*)(cache + i), cut, T()) << x * kVec;
+        else
+          for (int j = 0; j < kVec && i + j < n; j++) in |= (Bits)(at(i + j) >= cut) << (x * kVec + j);
       }
+      return in;
     };
     uint32_t mine = 0;
-    for (int s = s0; s < s1; s++) {
-      float v[kVec];
-      lane_values(s, v);
-#pragma unroll
-      for (int j = 0; j < kVec; j++) mine += v[j] >= cut;
-    }
-    const uint32_t of_warp = __reduce_add_sync(kFull, mine);
-    if (lane == 0) sh.warp_sum[warp] = of_warp;
+    for (int v = v0; v < v1; v += 8) mine += sizeof(Bits) == 8 ? __popcll(wanted(v)) : __popc((uint32_t)wanted(v));
+    uint32_t o = warp_inclusive32(mine);
+    if (lane == 31) sh.warp_sum[tid >> 5] = o;
     __syncthreads();
-    uint32_t o = 0, all = 0;  // where the warp's entries begin, the CTA's entries
+    o -= mine;
+    uint32_t all = 0;  // the CTA's entries; o: where this thread's begin
 #pragma unroll
     for (int w = 0; w < kSampWarps; w++) {
-      if (w < warp) o += (uint32_t)sh.warp_sum[w];
+      if (w < (tid >> 5)) o += (uint32_t)sh.warp_sum[w];
       all += (uint32_t)sh.warp_sum[w];
     }
     if (tid == 0) {
       sh.exchange[1] = all <= kListCap ? all : 1u << 30;
-      sh.first = all == 0 ? 0 : atomicAdd(&of(0)->few_n, all);
+      sh.first = all == 0 || all > kFewCap ? kFewCap : atomicAdd(&of(0)->few_n, all);
     }
-    __syncthreads();
     SampleShared* const to = of(0);
-    if (of_warp && all <= kListCap) {
-      const uint32_t first = sh.first;
-      const bool few = first < kFewCap && all <= kFewCap;
-      for (int s = s0; s < s1; s++) {
-        float v[kVec];
-        lane_values(s, v);
-        uint32_t in = 0;
-#pragma unroll
-        for (int j = 0; j < kVec; j++) in |= (uint32_t)(v[j] >= cut) << j;
-        if (!__any_sync(kFull, in != 0)) continue;
-        const uint32_t incl = (uint32_t)warp_inclusive32(__popc(in));
-        uint32_t at_ = o + incl - __popc(in);
-#pragma unroll
-        for (int j = 0; j < kVec; j++)
-          if (in >> j & 1) {
-            const int id = base + s * kStep + lane * kVec + j;
-            if (few && first + at_ < kFewCap) {
-              to->few_v[first + at_] = v[j];
-              to->few_i[first + at_] = id;
-            }
-            sh.list_v[at_] = v[j];
-            sh.list_i[at_++] = id;
+    if (all <= kFewCap) __syncthreads();
+    if (mine && all <= kListCap) {
+      const uint32_t first = all <= kFewCap ? sh.first : kFewCap;
+      for (int v = v0; v < v1; v += 8)
+        for (Bits in = wanted(v); in; in &= in - 1) {
+          const int i = v * kVec + (sizeof(Bits) == 8 ? __ffsll(in) : __ffs((uint32_t)in)) - 1;
+          const float x = at(i);
+          if (first + o < kFewCap) {
+            to->few_v[first + o] = x;
+            to->few_i[first + o] = base + i;
           }
-        o += __shfl_sync(kFull, incl, 31);
-      }
+          sh.list_v[o] = x;
+          sh.list_i[o++] = base + i;
+        }
     }
     cl.sync();  // rank 0's slice is not needed any more if the lists fit
     const u64 entries = over_cluster(1);
@@ -561,26 +567,33 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
   auto level = [&](uint32_t lo, uint32_t hi, int shift, bool by_count, Found above, uint32_t k_target,
                    double p_target, bool tail) {
     const bool again = lo == built_lo && hi == built_hi;
+    const bool single = shift == 0;  // a key a bin: its weight is that of one entry, times the count
     built_lo = lo;
     built_hi = hi;
     __syncthreads();
     if (!again)
-      for (int b = tid; b < kBins; b += kSampThreads) sh.count[b] = sh.m0[b] = sh.m1[b] = sh.m2[b] = 0;
+      for (int b = tid; b < kBins; b += kSampThreads) {
+        sh.count[b] = 0;
+        if (!single) sh.m0[b] = sh.m1[b] = sh.m2[b] = 0;
+      }
     if (tid == 0) sh.found = Found{-1, 0, 0, 0, 0};
     __syncthreads();
 #pragma unroll 4
     for (int i = tid; i < (again ? 0 : dn); i += kSampThreads) {
       const float v = value(i);
       const uint32_t kv = Key<T>::of(v);
-      const u64 f = kv < lo || kv > hi ? 0 : fixed(weight(v));
-      if (f) {
-        const int b = (int)((hi - kv) >> shift);
+      if (kv < lo || kv > hi) continue;
+      const int b = (int)((hi - kv) >> shift);
+      if (single) {
+        atomicAdd(&sh.count[b], 1u);
+      } else if (const u64 f = fixed(weight(v))) {
         atomicAdd(&sh.count[b], 1u);
         atomicAdd(&sh.m0[b], (uint32_t)f & 0x7FFF);
         atomicAdd(&sh.m1[b], (uint32_t)(f >> 15) & 0x7FFF);
         atomicAdd(&sh.m2[b], (uint32_t)(f >> 30));
       }
     }
+    auto key_mass = [&](int b) { return fixed(weight(Key<T>::value(hi - (uint32_t)b))); };  // (hi - b >= lo)
     if (local) {
       __syncthreads();
       u64 c[2], f[2];
@@ -588,7 +601,13 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
       for (int e = 0; e < 2; e++) {
         const int b = 2 * tid + e;
         c[e] = sh.count[b];
-        f[e] = (u64)sh.m0[b] + ((u64)sh.m1[b] << 15) + ((u64)sh.m2[b] << 30);
+        if (single) {
+          const u64 one = c[e] ? key_mass(b) : 0;
+          f[e] = one * c[e];
+          if (!one) c[e] = 0;
+        } else {
+          f[e] = (u64)sh.m0[b] + ((u64)sh.m1[b] << 15) + ((u64)sh.m2[b] << 30);
+        }
       }
       u64 ci = block_inclusive(c[0] + c[1], sh.warp_sum) + above.above - c[0] - c[1];
       u64 fi = block_inclusive(f[0] + f[1], sh.warp_sum) + above.mass_above - f[0] - f[1];
@@ -614,12 +633,17 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
         for (int r = i & 3; r < R; r += 4) {
           const SampleShared* o = of(r);
           c += o->count[g];
-          f += (u64)o->m0[g] + ((u64)o->m1[g] << 15) + ((u64)o->m2[g] << 30);
+          if (!single) f += (u64)o->m0[g] + ((u64)o->m1[g] << 15) + ((u64)o->m2[g] << 30);
         }
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
           c += __shfl_xor_sync(kFull, c, o);
           f += __shfl_xor_sync(kFull, f, o);
+        }
+        if (single) {
+          const u64 one = c ? key_mass(g) : 0;
+          f = one * c;
+          if (!one) c = 0;
         }
         if ((i & 3) == 0) {
           sh.bin_count[i >> 2] = c;
@@ -806,8 +830,8 @@ cudaError_t launch(const SampleArgs& args, cudaStream_t s) {
   SampleArgs a = args;
   // CTAs per row: slices of which two fit an SM (76 KB beside the 36 KB of tables), so that one
   // CTA's barriers and passes overlap another's; more, up to 16 and down to 2,048 entries each,
-  // while the rows leave SMs idle.  256 rows of 151,936 in bf16: 162 us with 4 CTAs a row, 195 with
-  // 2, 213 with 8.
+  // while the rows leave SMs idle.  256 rows of 151,936 in bf16: 133 us with 4 CTAs a row, 148 with
+  // 2, 181 with 8.
   int cluster = 1;
   while (cluster < 8 && (int64_t)a.vocab * (int)sizeof(T) > (int64_t)cluster * 76 * 1024) cluster *= 2;
   while (cluster < kMaxCluster && a.vocab > cluster * 4096 && (int64_t)a.rows * cluster * 2 <= 2 * kAttnSms) cluster *= 2;

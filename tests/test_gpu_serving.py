@@ -658,6 +658,21 @@ def test_sample_unusual_values():
     assert serving.sample(logits, greedy, hot)[0].tolist()[2:4] == [1, 1]
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_sample_steps_without_a_finite_factor(dtype):
+    """Infinite maxima, and temperatures whose reciprocal times the histogram's steps is beyond fp32."""
+    rng = np.random.RandomState(12)
+    logits = torch.from_numpy(rng.standard_normal((8, 40000)).astype(np.float32))
+    endless = logits.to(dtype)
+    endless[:, 17::97] = math.inf
+    endless[:, 5::89] = math.nan
+    u = rng.random_sample(8).astype(np.float32)
+    for k, p in ((None, None), ([3] * 8, None), ([700] * 8, [0.9] * 8), ([20000] * 8, [0.5] * 8), (None, [0.9] * 8)):
+        check_rows(endless.cuda(), u, None, k, p)
+        if dtype != F16:  # (fp16 has no such values)
+            check_rows((logits * 1e-37).to(dtype).cuda(), u, [1e-37] * 8, k, p)
+
+
 def test_sample_masked_logits():
     """Rows whose entries are masked with the type's lowest value, or -1e9 as the engine's early exit leaves them."""
     rng = np.random.RandomState(8)
