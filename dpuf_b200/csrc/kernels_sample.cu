@@ -40,7 +40,7 @@ constexpr int kSampThreads = 512;
 constexpr int kSampWarps = kSampThreads / 32;
 constexpr int kBins = 1024;
 constexpr int kMaxCluster = 16;
-constexpr int kListCap = 3072;            // entries that one CTA hands over
+constexpr int kListCap = 3 * kBins;       // entries that one CTA hands over (in the histograms' place)
 constexpr int kFewCap = 256;              // entries that are ranked by comparison
 constexpr float kFix = 8796093022208.0f;  // 2^43
 constexpr float kReach = 30.6f;           // > 44 ln 2: beyond it f is 0
