@@ -97,8 +97,8 @@ struct SampleShared {
     };
   };
   float few_v[kFewCap];  // in rank 0: the entries in no order,
-  int few_i[kFewCap];    // ranked ones' weights
-  u64 few_f[kFewCap], few_x[kFewCap];
+  int few_i[kFewCap];
+  u64 few_f[kFewCap], few_x[kFewCap];  // their weights; their places in the order
   unsigned few_n;
   uint32_t first;  // where this CTA's entries go
   uint32_t seg_count;
@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
     if (tid == 0) {
       sh.step_k = sh.step_p = kBins;
       sh.step_lo = 0;
+      sh.hi_k = sh.hi_m = 0.0f;
     }
     __syncthreads();
     float all_lo = 0.0f;
@@ -379,7 +380,9 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_rows_kernel(const __gr
     // running sums at the ends of bins 2 tid and 2 tid + 1
     const uint32_t run[2] = {cc - c[1], cc};
     const float run_lo[2] = {sl - lo[1], sl}, run_hi[2] = {sh_ - hi[1], sh_};
-    const int step_m = min_p > 0.0f ? min((int)(-logf(min_p) * per_step * 1.0001f) + 1, kBins - 1) : kBins - 1;
+    // bounded before it becomes an integer: a flat row's steps are so narrow that it may pass 2^31
+    const int step_m =
+        min_p > 0.0f ? (int)fminf(-logf(min_p) * per_step * 1.0001f, (float)(kBins - 2)) + 1 : kBins - 1;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       if (limit_k && run[e] > (uint32_t)k && run[e] - c[e] <= (uint32_t)k) {  // strictly more than k up to here

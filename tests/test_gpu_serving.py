@@ -686,6 +686,28 @@ def test_sample_masked_logits():
             check_rows(logits.cuda(), u, None, k, p)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [3000, 20000, 151936])  # 1, 8 and 16 CTAs a row
+def test_sample_flat_rows_with_min_p(dtype, vocab):
+    """Equal and nearly equal logits, and very high temperatures: the histogram's steps are then so narrow that
+    -ln(min_p) of them are more than an integer counts.  top_p ends half an entry's weight from the next (the
+    fp32 weights' error adds up to 2^-24 vocab < 0.01 of one)."""
+    rows, k = 6, vocab // 3
+    rng = np.random.RandomState(vocab)
+    u = rng.random_sample(rows).astype(np.float32)
+    share = lambda p, n: [(math.floor(p * n) + 0.5) / n] * rows  # noqa: E731
+    near = torch.from_numpy(rng.randint(0, 3, (rows, vocab)).astype(np.float32)) * 2.0 ** -20
+    same = torch.zeros(rows, vocab)
+    spread = torch.from_numpy(rng.standard_normal((rows, vocab)).astype(np.float32))
+    for logits, temp in ((same, None), (same - 1e4, None), (near, None), (near + 1, None), (spread, 1e7), (spread, 1e30)):
+        logits, temp = logits.to(dtype).cuda(), None if temp is None else [temp] * rows
+        for m in (1e-30, 0.05) if temp else (1e-30, 0.05, 0.2, 1.0):  # (hot weights may round to 1)
+            check_rows(logits, u, temp, None, share(0.9, vocab), [m] * rows)
+        check_rows(logits, u, temp, [k] * rows, None, [0.05] * rows)
+        check_rows(logits, u, temp, [k] * rows, share(0.7, k), [0.05] * rows)
+        check_rows(logits, u, temp, None, None, [0.05] * rows)
+
+
 def test_sample_strided_rows():
     rng = np.random.RandomState(9)
     wide = torch.from_numpy(rng.standard_normal((6, 5003)).astype(np.float32)).half().cuda()
