@@ -750,6 +750,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         if (p.a.out_dtype == DPUF_TYPE_F32) write(std::true_type());
         else write(std::false_type());
       }
+      // what this thread wrote to and read from the queries' shared memory comes before the TMA load
+      // of the item after next into it
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
         if (alone) bar_arrive(q_done);

@@ -332,6 +332,22 @@ def test_attention_many_items_a_cta(dtype, heads, q_lens, hd):
     run_attention((dtype, dtype), heads, hd, 16, q, kv, repeats=30)
 
 
+@pytest.mark.parametrize("heads,q_lens", [((8, 2), [40, 9]), ((8, 2), [64, 128, 31]), ((3, 3), [256, 127]), ((16, 1), [16, 5])],
+                         ids=str)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_results_by_way_of_the_queries_buffer(heads, q_lens, hd, wide):
+    """Partial tiles, and all tiles of fp32 results, pass through the shared memory that the queries of the item
+    after next arrive in: many items a CTA, queries by TMA (the group divides 128)."""
+    rng = np.random.RandomState(hd)
+    q = [q_lens[i % len(q_lens)] for i in range(400)]
+    kv = [n + rng.randint(0, 20) for n in q]
+    out = torch.empty(sum(q), heads[0], hd, dtype=F32, device="cuda") if wide else None
+    got = run_attention((F16, F16), heads, hd, 16, q, kv, out=out, repeats=0 if wide else 20)
+    if wide:  # rounded once more it is the narrow result
+        assert torch.equal(got.half(), run_attention((F16, F16), heads, hd, 16, q, kv, repeats=20))
+
+
 @pytest.mark.parametrize("heads,seqs,q_len,kv_len", [((3, 3), 49, 216, 216), ((3, 3), 58, 216, 300), ((4, 2), 20, 70, 900),
                                                       ((4, 1), 37, 100, 1100), ((2, 2), 41, 257, 777), ((8, 2), 1, 333, 2500)])
 def test_attention_cuts_at_item_ends(heads, seqs, q_len, kv_len):
