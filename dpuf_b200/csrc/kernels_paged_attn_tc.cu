@@ -30,8 +30,10 @@
 // Results leave by way of the queries' shared memory: a row is a thread's, and 32 rows' pieces in
 // one store cost a cycle a row.
 //
-// Every wait is bounded: one that gives up sets the workspace's error word and the CTA's abort
-// flag, all roles stop, copies in flight are waited for (bounded) and TMEM is freed.
+// Every wait on an mbarrier is bounded: one that gives up sets the workspace's error word and the
+// CTA's abort flag, all roles stop, copies in flight are waited for (bounded) and TMEM is freed.  A
+// tile's softmax warps wait each for itself, so they agree on whether one gave up (once an item)
+// before they go on to the barriers that need all four.
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -527,6 +529,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
     };
     bool ok = true;
     auto wg_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory"); };
+    // Whether none of the tile's four warps gave up a wait: they leave together or meet at every wg_sync.
+    auto agree = [&](bool mine) {
+      int all;
+      asm volatile(
+          "{ .reg .pred p, q; setp.ne.b32 p, %2, 0; bar.red.and.pred q, %1, 128, p; selp.s32 %0, 1, 0, q; }"
+          : "=r"(all)
+          : "r"(1 + w), "r"((int)mine)
+          : "memory");
+      return all != 0;
+    };
     for (int left = run.n; ok && left > 0;) {
       int from, to;
       const int done = run.n - left;
@@ -616,7 +628,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
         bar_arrive(&p_full[w][h]);
         stored();  // the item before's, long read by now
       }
-      if (!ok || !(ok = warp_wait(&pv_done[w][(blocks - 1) & 1], (blocks - 1) >> 1 & 1, give))) break;
+      if (ok) ok = warp_wait(&pv_done[w][(blocks - 1) & 1], (blocks - 1) >> 1 & 1, give);
+      if (!(ok = agree(ok))) break;
       fence_after();
 
       // ---- the whole item, or a part of it
