@@ -5,7 +5,8 @@
 //   m' = max(m, max s_j),  p_j = exp(s_j - m'),  l' = l e^{m-m'} + sum p_j,
 //   o' = o e^{m-m'} + sum p_j v_j,  at the end out = o / l (0 where l = 0).
 // Scores are kept in units of log 2 (scale * log2(e) is folded into the product), so every
-// exponential is one ex2.  A row that has seen nothing has m = -inf and l = 0.
+// exponential is one ex2.  A row that has seen nothing has m = -inf and l = 0.  A score that is NaN
+// does not raise m, but makes l and o NaN; they stay that whatever they are multiplied by.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -105,10 +106,12 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
       float top = fmaxf(s0, s1);
 #pragma unroll
       for (int i = 8; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, i));
-      const float m2 = fmaxf(m, top);
-      if (m2 != -CUDART_INF_F) {
-        const float f = ex2(m - m2);
-        const float p0 = ex2(s0 - m2), p1 = ex2(s1 - m2);
+      const bool sees = j0 < hi && j0 + kGenKeys > lo;  // this row, of the block
+      if (sees) {
+        // (a NaN score does not raise the maximum, but reaches l and o: the factors are never skipped)
+        const float m2 = fmaxf(m, top), ref = m2 == -CUDART_INF_F ? 0.0f : m2;
+        const float f = m == -CUDART_INF_F ? 0.0f : ex2(m - m2);
+        const float p0 = ex2(s0 - ref), p1 = ex2(s1 - ref);
         ps[row * (kGenKeys + 1) + x] = p0;
         ps[row * (kGenKeys + 1) + x + 16] = p1;
         l = fmaf(l, f, p0 + p1);  // this thread's keys only; summed over the row at the end
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
           for (int e = 0; e < 4; e++) o[i][e] *= f;
       }
       __syncwarp();
-      if (m != -CUDART_INF_F)
+      if (sees)
         for (int k = 0; k < kGenKeys; k++) {
           const float w = ps[row * (kGenKeys + 1) + k];
 #pragma unroll
@@ -157,25 +160,24 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
         for (int i = 0; i < DP / 64; i++)
 #pragma unroll
           for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
-        if (m != -CUDART_INF_F)
-          for (int cc = c0; cc <= c1; cc++) {
-            const size_t at = (2 * (size_t)cc + (cc == c0 ? 1 : 0)) * kGenRows + row;
-            const float2 part = __ldcg(&parts.ml[at]);
-            const float f = ex2(part.x - m);
-            l = fmaf(part.y, f, l);
+        for (int cc = c0; cc <= c1; cc++) {
+          const size_t at = (2 * (size_t)cc + (cc == c0 ? 1 : 0)) * kGenRows + row;
+          const float2 part = __ldcg(&parts.ml[at]);
+          const float f = part.x == -CUDART_INF_F ? 0.0f : ex2(part.x - m);
+          l = fmaf(part.y, f, l);
 #pragma unroll
-            for (int i = 0; i < DP / 64; i++) {
-              const float4 v = __ldcg((const float4*)(parts.o + at * DP + 64 * i + 4 * x));
-              o[i][0] = fmaf(v.x, f, o[i][0]);
-              o[i][1] = fmaf(v.y, f, o[i][1]);
-              o[i][2] = fmaf(v.z, f, o[i][2]);
-              o[i][3] = fmaf(v.w, f, o[i][3]);
-            }
+          for (int i = 0; i < DP / 64; i++) {
+            const float4 v = __ldcg((const float4*)(parts.o + at * DP + 64 * i + 4 * x));
+            o[i][0] = fmaf(v.x, f, o[i][0]);
+            o[i][1] = fmaf(v.y, f, o[i][1]);
+            o[i][2] = fmaf(v.z, f, o[i][2]);
+            o[i][3] = fmaf(v.w, f, o[i][3]);
           }
+        }
       }
     }
     if ((whole || join) && live) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
       const size_t at = ((size_t)(c.seq.q0 + tok) * p.a.n_q + head) * hd;
 #pragma unroll
       for (int i = 0; i < DP / 64; i++)

@@ -301,6 +301,39 @@ def test_attention_empty_rows(types, q_lens):
 
 
 @pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q_len", [1, 6, 200])
+@pytest.mark.parametrize("before", [102, 9102])  # positions before the new tokens: one part, several
+def test_attention_values_that_are_not_finite(types, hd, q_len, before):
+    """A NaN or infinite query gives NaN in its own row alone; a NaN key in every row that sees it, also where it is
+    all that the row sees of a block of keys (position 63 of a window of 40 that begins there)."""
+    g = gen(hd + q_len)
+    dtype, kv_dtype = types
+    total, hq, hkv = before + q_len, 8, 2
+    table, n_pages = table_for([total], 16, g)
+    k, v = (normal(g, n_pages, hkv, 16, hd, dtype=kv_dtype) for _ in range(2))
+    cache = serving.PagedCache(k, v)
+    q = normal(g, q_len, hq, hd, dtype=dtype)
+    start, kv = torch.tensor([0, q_len], dtype=INT, device="cuda"), torch.tensor([total], dtype=INT, device="cuda")
+    want, bound = attention64(cache, table, q, [0, q_len], [total], hd ** -0.5, True, 0)
+    token = q_len // 2
+    for value, dim in ((math.nan, 0), (math.inf, hd - 1), (-math.inf, 5)):
+        bad = q.clone()
+        bad[token, 3, dim] = value  # (of the 100 keys and more that it sees, some have a score of +infinity)
+        got = serving.paged_attention(cache, table, bad, start, kv, q_len)
+        assert bool(got[token, 3].isnan().all()), value
+        got[token, 3] = want[token, 3].to(got.dtype)
+        assert bool(((got.double() - want).abs() <= bound).all()), value
+    for at, window in ((0, 0), (before - 39, 40)):
+        held = k[table[0, at // 16].long(), 1, at % 16].clone()
+        k[table[0, at // 16].long(), 1, at % 16] = math.nan
+        got = serving.paged_attention(cache, table, q, start, kv, q_len, window=window)
+        k[table[0, at // 16].long(), 1, at % 16] = held
+        sees = at - before + window if window else q_len  # tokens t < sees: at > before + t - window
+        assert bool(got[:sees, 4:].isnan().all()), window
+
+
+@pytest.mark.parametrize("types", TYPES, ids=str)
 @pytest.mark.parametrize("junk", [math.inf, -math.inf, 6e4])
 def test_attention_unused_places(types, junk):
     run_attention(types, (8, 2), 64, 32, [1, 77, 1], [45, 201, 3], junk=junk)
