@@ -10,6 +10,7 @@ namespace dpuf {
 
 constexpr int kAttnSms = 148;
 constexpr int kAttnHeader = 256;  // the error word
+static_assert(kAttnHeader + kAttnCounterBytes <= DPUF_PAGED_ATTENTION_ZEROED, "what is zero before the first use");
 
 // Set to 1 when a bounded wait gave up.
 DPUF_HD int* attn_error(void* ws) { return (int*)ws; }

@@ -118,6 +118,16 @@ DPUF_EXPORT int32_t dpuf_cuda_paged_attention_status(void* workspace, void* stre
   return -6;
 }
 
+DPUF_EXPORT uint64_t dpuf_cuda_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();  // not left for the next call to find
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 DPUF_EXPORT int32_t dpuf_cuda_sample_rows(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
                                           int32_t vocab, const float* u, const float* temperature,
                                           const int32_t* top_k, const float* top_p, const float* min_p,

@@ -4,10 +4,15 @@ fused with the cache's append, attention of new tokens over the cache, and sampl
 They run in libdpuf_cuda.so (`dpuf_cuda_rope_append`, `dpuf_cuda_paged_attention`,
 `dpuf_cuda_sample_rows` in include/dpuf_cuda.h, which also states the formulas); this module
 checks arguments, allocates outputs and passes device pointers.  Calls enqueue on torch's current
-stream of the tensors' device, do not synchronise, and can be captured in a CUDA graph (make the
-first `paged_attention` call of a stream before capturing on it: it sets up the stream's
-workspace).  Arguments that do not fit raise ValueError or TypeError, a failed launch RuntimeError.
-There is no fallback.
+stream of the tensors' device, do not synchronise, and can be captured in a CUDA graph.  Arguments
+that do not fit raise ValueError or TypeError, a failed launch RuntimeError.  There is no fallback.
+
+`paged_attention` needs a workspace (39 MB), and calls that share one must not overlap.  Without one
+given, a call uses that of the current stream, whose calls follow each other (kept for as long as the
+program runs), and a call that `torch.cuda.graph` captures one that its graph has for itself: graphs
+may be replayed on any streams, at once too (except where they share a memory pool).  A program that
+captures in another way, or wants `attention_check` to see a graph's calls, passes its own from
+`attention_workspace`.
 
 One decoding step of a batch, per layer and at its end:
 
@@ -34,7 +39,9 @@ _INT = torch.int32
 _FLOAT = torch.float32
 
 _typed = None
-_workspaces: dict = {}  # (device, stream) -> zeroed workspace of paged_attention
+_workspaces: dict = {}  # (device, stream) -> workspace of paged_attention (tensor, address, bytes)
+_captured: dict = {}    # (device, stream) -> (capture, such a workspace) of the graph captured on it last
+_ZEROED = 8192          # DPUF_PAGED_ATTENTION_ZEROED
 
 
 def _lib():
@@ -49,6 +56,8 @@ def _lib():
         lib.dpuf_cuda_paged_attention_workspace.argtypes = []
         lib.dpuf_cuda_paged_attention_status.restype = ctypes.c_int32
         lib.dpuf_cuda_paged_attention_status.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        lib.dpuf_cuda_stream_capture_id.restype = ctypes.c_uint64
+        lib.dpuf_cuda_stream_capture_id.argtypes = [ctypes.c_void_p]
         lib.dpuf_cuda_sample_rows.restype = ctypes.c_int32
         lib.dpuf_cuda_sample_rows.argtypes = ([ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int32,
                                                ctypes.c_int32] + [ctypes.c_void_p] * 8)
@@ -59,6 +68,7 @@ def _lib():
 # torch.cuda.current_stream() and current_device() build objects; these return the numbers
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
+_capturing = torch.cuda.is_current_stream_capturing
 _raw_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
@@ -227,22 +237,47 @@ def rope_append(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor, k:
     return out
 
 
+def attention_workspace(device: int | None = None) -> torch.Tensor:
+    """A workspace for `paged_attention`'s calls, made on the current stream of the device."""
+    dev = torch.cuda.current_device() if device is None else device
+    ws = torch.empty(_lib().dpuf_cuda_paged_attention_workspace(), dtype=torch.uint8, device=f"cuda:{dev}")
+    ws[:_ZEROED].zero_()
+    return ws
+
+
+def _given(ws: torch.Tensor, device: int) -> tuple:
+    _check(ws, "workspace", torch.uint8, device, 1)
+    if ws.data_ptr() % 16 or ws.numel() < _lib().dpuf_cuda_paged_attention_workspace():
+        raise ValueError("workspace is not one of attention_workspace()")
+    return ws, ws.data_ptr(), ws.numel()
+
+
 def _workspace(device: int) -> tuple:
-    """The current stream's workspace (tensor, address, bytes): calls on one stream follow each other, so they can share it."""
-    key = (device, _raw_stream(device))
+    """The workspace (tensor, address, bytes) of the current stream, or of the capture that it is in."""
+    stream = _raw_stream(device)
+    key = (device, stream)
+    if _raw_device() != device or _capturing():  # (it asks the current device's stream)
+        capture = _lib().dpuf_cuda_stream_capture_id(stream)
+        if capture:
+            found = _captured.get(key)
+            # held until the stream's next call after the capture: the graph's pool has the memory, and
+            # nothing else captured into the graph may get it
+            if found is None or found[0] != capture:
+                ws = attention_workspace(device)
+                found = _captured[key] = (capture, (ws, ws.data_ptr(), ws.numel()))
+            return found[1]
+    if _captured:
+        _captured.pop(key, None)
     found = _workspaces.get(key)
     if found is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("call paged_attention once on this stream before capturing it")
-        n = _lib().dpuf_cuda_paged_attention_workspace()
-        ws = torch.zeros(n, dtype=torch.uint8, device=f"cuda:{device}")
-        found = _workspaces[key] = (ws, ws.data_ptr(), n)
+        ws = attention_workspace(device)
+        found = _workspaces[key] = (ws, ws.data_ptr(), ws.numel())
     return found
 
 
 def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor, q_start: torch.Tensor,
                     kv_len: torch.Tensor, max_q: int, scale: float | None = None, causal: bool = True, window: int = 0,
-                    out: torch.Tensor | None = None) -> torch.Tensor:
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q `[tokens, n_q, head_dim]` over the cache; returns `[tokens, n_q, head_dim]`.
 
     Sequence s (row s of page_table) has the new tokens q_start[s] .. q_start[s + 1] (int32
@@ -252,7 +287,8 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
     n_q is a multiple of the cache's heads.  q is float32 or of the cache's type and may be a slice
     (the last dimension contiguous, strides multiples of 16 bytes).  scale defaults to
     head_dim^-0.5.  The result is `out` (contiguous; q's type or float32) or a new tensor of q's
-    type."""
+    type.  workspace is one of `attention_workspace` that no call or replay in flight uses; without it
+    the call uses its stream's, or its graph's."""
     dev = cache.device_index
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         raise ValueError("q must be [tokens, n_q, head_dim] with the cache's head_dim")
@@ -279,7 +315,7 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
         raise ValueError("out must be contiguous, of q's shape and on its device")
     elif out.dtype != q.dtype and out.dtype != _FLOAT:
         raise TypeError("out must be float32 or of q's type")
-    _, ws, ws_bytes = _workspace(dev)
+    _, ws, ws_bytes = _workspace(dev) if workspace is None else _given(workspace, dev)
     args = cache._packed + _ATTN.pack(
         page_table.data_ptr(), page_table.stride(0), q.data_ptr(), qs[0], qs[1], out.data_ptr(), q_start.data_ptr(),
         kv_len.data_ptr(), ws, ws_bytes, n_seqs, width, n, n_q, max_q, bool(causal), window, code,
@@ -288,11 +324,12 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
     return out
 
 
-def attention_check(device: int | None = None) -> None:
-    """Waits for the current stream and raises RuntimeError if a bounded wait inside one of its
-    `paged_attention` calls gave up since the last check (that call's output is undefined)."""
+def attention_check(device: int | None = None, workspace: torch.Tensor | None = None) -> None:
+    """Waits for the current stream and raises RuntimeError if a bounded wait inside a `paged_attention`
+    call on the workspace (without one, the stream's) gave up since the last check: the outputs of that
+    call and of those after it are undefined.  The workspace is then ready for use again."""
     dev = torch.cuda.current_device() if device is None else device
-    _call(_lib().dpuf_cuda_paged_attention_status, dev, _workspace(dev)[1])
+    _call(_lib().dpuf_cuda_paged_attention_status, dev, (_workspace(dev) if workspace is None else _given(workspace, dev))[1])
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None,

@@ -223,8 +223,12 @@ DPUF_EXPORT int32_t dpuf_cuda_rope_append(const DpufRopeAppendArgs* args, void* 
  * [n_tokens][n_q][head_dim] (contiguous) and is dtype or float32.  Positions that no token of a
  * sequence sees are never used, whatever stands there; a value that is not finite at a position
  * below kv_len[s] may reach every row of that sequence.
- * workspace: dpuf_cuda_paged_attention_workspace() bytes, 16-byte aligned, all zero before its
- * first use (each call leaves its counters at zero); calls that share one must not overlap. */
+ * workspace: dpuf_cuda_paged_attention_workspace() bytes, 16-byte aligned, the first
+ * DPUF_PAGED_ATTENTION_ZEROED of them zero before its first use (each call leaves its counters at
+ * zero).  Calls that share one must not overlap, and a call in a CUDA graph uses the one it was
+ * captured with whichever stream replays it: give a graph a workspace of its own, or order its
+ * replays with all other uses. */
+enum { DPUF_PAGED_ATTENTION_ZEROED = 8192 };
 typedef struct DpufPagedAttentionArgs {
   DpufPagedKv kv;
   const int32_t* page_table; /* [n_seqs][table_stride], pages_per_seq entries used */
@@ -241,9 +245,12 @@ typedef struct DpufPagedAttentionArgs {
 DPUF_EXPORT int64_t dpuf_cuda_paged_attention_workspace(void);
 DPUF_EXPORT int32_t dpuf_cuda_paged_attention(const DpufPagedAttentionArgs* args, void* stream);
 /* Waits for `stream` and says whether every wait inside the kernels that used the workspace was
- * met: 0, or -6 if one gave up (2 s; that call's output is undefined; the workspace is then made
- * ready for use again), -1 or -4 as above. */
+ * met: 0, or -6 if one gave up (2 s; the outputs of that call and of those after it on this
+ * workspace are undefined; it is then made ready for use again), -1 or -4 as above. */
 DPUF_EXPORT int32_t dpuf_cuda_paged_attention_status(void* workspace, void* stream);
+/* The number of the graph capture that `stream` is in (never 0), 0 where it is in none or cannot be
+ * asked. */
+DPUF_EXPORT uint64_t dpuf_cuda_stream_capture_id(void* stream);
 
 /* Sampling on the device: one token per row of logits [rows][vocab] (row stride row_stride
  * elements, vocab <= 2^20, dtype DPUF_TYPE_*) from the given uniforms u[rows] in [0, 1).

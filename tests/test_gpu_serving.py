@@ -493,6 +493,84 @@ def test_attention_on_streams_and_in_a_graph(q_len):
     assert torch.equal(want, out)
 
 
+@pytest.mark.parametrize("q_len", [1, 100])
+def test_attention_graph_keeps_off_its_streams_workspace(q_len):
+    """A graph's calls share nothing with later calls on the stream that it was captured on."""
+    args = attention_inputs(q_len)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        want = serving.paged_attention(*args)
+        out = torch.zeros_like(want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            serving.paged_attention(*args, out=out)
+    held = [w[0] for key, w in serving._workspaces.items() if key[1] == s.cuda_stream]
+    torch.cuda.synchronize()
+    assert len(held) == 1
+    held[0][256:5000] = 255  # as another call in flight may have them: the counters
+    graph.replay()  # (once: a second call would find the first one's parts of the same inputs)
+    torch.cuda.synchronize()
+    held[0][256:5000] = 0
+    assert torch.equal(want, out)
+
+
+@pytest.mark.parametrize("q_len", [1, 100])
+@pytest.mark.parametrize("given", [False, True])
+def test_attention_graphs_of_one_stream_on_two(q_len, given):
+    """Graphs captured one after the other on one stream, replayed on two at once while the first is in use too."""
+    home, others = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    sets = [attention_inputs(q_len, seqs) for seqs in (5, 9, 14)]
+    want = [serving.paged_attention(*args) for args in sets]
+    torch.cuda.synchronize()
+    outs, graphs, spaces = [torch.zeros_like(w) for w in want], [], []
+    for args, out in zip(sets[:2], outs):
+        spaces.append(serving.attention_workspace() if given else None)
+        graphs.append(torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graphs[-1], stream=home):
+            for _ in range(3):
+                serving.paged_attention(*args, out=out, workspace=spaces[-1])
+    for _ in range(20):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, s in zip(graphs, others):
+                with torch.cuda.stream(s):
+                    g.replay()
+            with torch.cuda.stream(home):
+                serving.paged_attention(*sets[2], out=outs[2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    for ws in spaces:
+        if ws is not None:
+            serving.attention_check(workspace=ws)
+
+
+@pytest.mark.parametrize("q_len", [1, 100])
+def test_attention_workspace_after_a_wait_gave_up(q_len):
+    """The error word set and the counters left anywhere, as a kernel that gave up leaves them: the check says so
+    once and makes the workspace ready for use."""
+    args = attention_inputs(q_len)
+    want = serving.paged_attention(*args)
+    ws = serving.attention_workspace()
+    for _ in range(2):
+        assert torch.equal(want, serving.paged_attention(*args, workspace=ws))
+        serving.attention_check(workspace=ws)
+        ws[:1] = 1
+        ws[256:5000:4] = 3
+        with pytest.raises(RuntimeError, match="gave up"):
+            serving.attention_check(workspace=ws)
+        serving.attention_check(workspace=ws)
+    for error, bad in ((TypeError, ws.view(torch.int32)), (ValueError, ws[:-1]), (ValueError, ws.cpu()),
+                       (ValueError, torch.zeros(ws.numel() + 1, dtype=torch.uint8, device="cuda")[1:]),
+                       (ValueError, ws[None]), (ValueError, torch.zeros(2 * ws.numel(), dtype=torch.uint8, device="cuda")[::2])):
+        with pytest.raises(error):
+            serving.paged_attention(*args, workspace=bad)
+        with pytest.raises(error):
+            serving.attention_check(workspace=bad)
+
+
 def test_attention_lengths_that_do_not_fit():
     """Lengths and starts are read on the device: ones beyond the table or the tokens are cut off."""
     cache, table, q, start, kv, _ = attention_inputs()
