@@ -274,6 +274,20 @@ DPUF_DEV void attn_owners(const AttnRun& r, const AttnCursor& c, int* c0, int* c
   *c1 = holds(c.begin + hi - 1);
 }
 
+// Zeros for the tokens before the first sequence's and after the last one's (padding of a batch): each
+// CTA takes some of them.
+DPUF_DEV void attn_zero_unowned(const AttnArgs& p) {
+  const int n = p.a.n_tokens;
+  const int first = min(max(p.a.q_start[0], 0), n), end = max(min(p.a.q_start[p.a.n_seqs], n), first);
+  const int rows = first + n - end;
+  if (rows == 0) return;
+  const int64_t bytes = (int64_t)p.a.n_q * p.a.kv.head_dim * (p.a.out_dtype == DPUF_TYPE_F32 ? 4 : 2);  // 16 k
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    uint4* const row = (uint4*)((char*)p.a.out + (r < first ? r : r - first + end) * bytes);
+    for (int64_t i = threadIdx.x; i < bytes / 16; i += blockDim.x) row[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // Cache offset (elements) of head 0, row 0 of the page that holds position j of sequence s, or -1.
 DPUF_DEV int64_t attn_page(const AttnArgs& p, int s, int j) {
   const int page = p.a.page_table[(size_t)s * p.a.table_stride + (j >> p.page_shift)];

@@ -46,6 +46,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attention_f32_kernel(const 
   const int tid = threadIdx.x, row = tid >> 4, x = tid & 15;
   const int hd = p.a.kv.head_dim;
   AttnRun run = attn_locate<kGenRows, kGenKeys>(p, share, blockIdx.x, gridDim.x, kJoin);
+  attn_zero_unowned(p);
   if (run.n == 0) return;
   const AttnParts<kGenRows, DP> parts(p.a.workspace, gridDim.x);
   AttnCursor& c = run.cur;
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, few_ctas(DP)) paged_attention_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 3, gl = lane & 7;
   const int hd = p.a.kv.head_dim;
   AttnRun run = attn_locate<R, kFewKeys>(p, share, blockIdx.x, gridDim.x, kFewJoin);
+  attn_zero_unowned(p);
   if (run.n == 0) return;
   const AttnParts<R, DP> parts(p.a.workspace, gridDim.x);
   AttnCursor& c = run.cur;

@@ -95,6 +95,7 @@ paged_attention_rows_kernel(const __grid_constant__ AttnArgs p) {
   const int hd = p.a.kv.head_dim;
   const AttnParts<kRows, DP> parts(p.a.workspace, gridDim.x);
   AttnRun run = attn_locate<kRows, kKeys>(p, share, blockIdx.x, gridDim.x, kJoin / (float)min(kRows, p.a.max_q * p.group));
+  attn_zero_unowned(p);
   if (run.n == 0) return;
 
   // ---- the warp's stream of keys and values

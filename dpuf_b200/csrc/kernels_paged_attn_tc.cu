@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_tc_kernel(const _
   }
   fence_before();
   AttnRun run = attn_locate<kItemRows, kKeys, kLead, kSnap>(p, share, blockIdx.x, gridDim.x, kJoin);
+  attn_zero_unowned(p);
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_sh;

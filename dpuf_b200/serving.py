@@ -68,7 +68,8 @@ def _lib():
 # torch.cuda.current_stream() and current_device() build objects; these return the numbers
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
-_capturing = torch.cuda.is_current_stream_capturing
+_capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing") else (
+    torch.cuda.is_current_stream_capturing)
 _raw_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
@@ -281,8 +282,9 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
     """Attention of q `[tokens, n_q, head_dim]` over the cache; returns `[tokens, n_q, head_dim]`.
 
     Sequence s (row s of page_table) has the new tokens q_start[s] .. q_start[s + 1] (int32
-    `[sequences + 1]`, at most max_q each), which are the last of its kv_len[s] (int32) positions
-    and have been appended.  A token at position p sees the positions up to p (all kv_len[s] where
+    `[sequences + 1]`, ascending, at most max_q each), which are the last of its kv_len[s] (int32)
+    positions and have been appended; tokens before q_start[0] and from the last entry on are padding
+    and get zeros.  A token at position p sees the positions up to p (all kv_len[s] where
     not causal), with `window` > 0 the last `window` of them; one that sees nothing gets zeros.
     n_q is a multiple of the cache's heads.  q is float32 or of the cache's type and may be a slice
     (the last dimension contiguous, strides multiples of 16 bytes).  scale defaults to

@@ -213,9 +213,10 @@ typedef struct DpufRopeAppendArgs {
 DPUF_EXPORT int32_t dpuf_cuda_rope_append(const DpufRopeAppendArgs* args, void* stream);
 
 /* Attention of new tokens over the paged cache.  Sequence s has the new tokens q_start[s] ..
- * q_start[s+1] (q_start[0] = 0, q_start[n_seqs] = n_tokens), which are the last of its
- * kv_len[s] positions and are in the cache already.  The token at position p sees the positions
- * j <= p (all kv_len[s] if causal is 0), and with window > 0 only j > p - window;
+ * q_start[s+1] (ascending; tokens before q_start[0] and from q_start[n_seqs] on are padding, whose
+ * rows of out get zeros), which are the last of its kv_len[s] positions and are in the cache
+ * already.  The token at position p sees the positions j <= p (all kv_len[s] if causal is 0), and
+ * with window > 0 only j > p - window;
  *   out = sum_j softmax_j(scale * q . k_j) v_j,
  * zeros for a token that sees nothing.  Query head h reads KV head h / (n_q / n_kv).  max_q (at
  * least the largest q_start[s+1] - q_start[s]; rows beyond it are not written) chooses the

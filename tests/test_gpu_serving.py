@@ -571,6 +571,32 @@ def test_attention_workspace_after_a_wait_gave_up(q_len):
             serving.attention_check(workspace=bad)
 
 
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("q_len", [1, 6, 100])
+@pytest.mark.parametrize("hd", [64, 72, 136])
+def test_attention_rows_of_no_sequence(types, q_len, hd):
+    """Tokens before the first sequence's and after the last one's, as a padded batch has them, get zeros."""
+    g = gen(hd)
+    lens = [q_len + 90 * s for s in range(4)]
+    table, n_pages = table_for(lens, 16, g)
+    cache = serving.PagedCache(*(normal(g, n_pages, 3, 16, hd, dtype=types[1]) for _ in range(2)))
+    n = q_len * len(lens)
+    start = torch.arange(0, n + 1, q_len, dtype=INT, device="cuda")
+    kv = torch.tensor(lens, dtype=INT, device="cuda")
+    for before, after in ((0, 1), (3, 0), (2, 700)):
+        q = normal(g, before + n + after, 6, hd, dtype=types[0])
+        want = serving.paged_attention(cache, table, q[before : before + n], start, kv, q_len)
+        for out_type in {types[0], F32}:
+            out = torch.full_like(q, 7.0, dtype=out_type)
+            serving.paged_attention(cache, table, q, start + before, kv, q_len, out=out)
+            assert bool((out[:before] == 0).all()) and bool((out[before + n :] == 0).all())
+            assert torch.equal(out[before : before + n].to(types[0]), want)
+    nobody = torch.zeros(5, dtype=INT, device="cuda")  # all of them
+    out = torch.full_like(q, 7.0)
+    serving.paged_attention(cache, table, q, nobody, kv, q_len, out=out)
+    assert bool((out == 0).all())
+
+
 def test_attention_lengths_that_do_not_fit():
     """Lengths and starts are read on the device: ones beyond the table or the tokens are cut off."""
     cache, table, q, start, kv, _ = attention_inputs()
