@@ -127,25 +127,27 @@ def generate(paged: PagedModel, prompts, n_new: int, temperature: float = 0.0, t
     """n_new tokens after each prompt.  Prompts go in by chunks of at most `chunk` tokens, in the
     same steps in which the sequences that are past theirs generate."""
     g = torch.Generator(device="cuda").manual_seed(seed)
-    seqs = [paged.open() for _ in prompts]
     todo = [list(map(int, p)) for p in prompts]
+    seqs = [paged.open() for _ in prompts]
     out: list[list[int]] = [[] for _ in prompts]
-    while any(len(o) < n_new for o in out):
-        live = [i for i, o in enumerate(out) if len(o) < n_new]
-        batch = [(seqs[i], todo[i][:chunk]) for i in live]
-        logits = paged.step(batch)
-        for i in live:
-            todo[i] = todo[i][chunk:]
-        n = len(live)
-        full = lambda x, t: torch.full((n,), x, dtype=t, device="cuda")  # noqa: E731
-        ids, _ = serving.sample(logits, torch.rand(n, generator=g, device="cuda"), full(temperature, torch.float32),
-                                full(top_k, torch.int32), full(top_p, torch.float32), full(min_p, torch.float32))
-        for i, token in zip(live, ids.tolist()):
-            if not todo[i]:  # the prompt is in: this is its next token
-                out[i].append(token)
-                todo[i] = [token]
-    for s in seqs:
-        paged.close(s)
+    try:
+        while any(len(o) < n_new for o in out):
+            live = [i for i, o in enumerate(out) if len(o) < n_new]
+            batch = [(seqs[i], todo[i][:chunk]) for i in live]
+            logits = paged.step(batch)
+            for i in live:
+                todo[i] = todo[i][chunk:]
+            n = len(live)
+            full = lambda x, t: torch.full((n,), x, dtype=t, device="cuda")  # noqa: E731
+            ids, _ = serving.sample(logits, torch.rand(n, generator=g, device="cuda"), full(temperature, torch.float32),
+                                    full(top_k, torch.int32), full(top_p, torch.float32), full(min_p, torch.float32))
+            for i, token in zip(live, ids.tolist()):
+                if not todo[i]:  # the prompt is in: this is its next token
+                    out[i].append(token)
+                    todo[i] = [token]
+    finally:
+        for s in seqs:
+            paged.close(s)
     return out
 
 

@@ -71,6 +71,25 @@ def test_generate_frees_its_pages_and_repeats():
         paged.release()
 
 
+def test_generate_frees_its_pages_where_a_step_fails():
+    from dpuf_b200 import paged_serve
+
+    m = mdl.SyntheticModel(mdl.TINY, seed=2)
+    paged = paged_serve.PagedModel(m, 12)
+    try:
+        prompts = [mdl.prompt_ids(n, m.shape.vocab, n) for n in (3, 60, 20)]
+        for error, bad in ((ValueError, prompts + [[]]), (RuntimeError, prompts + [prompts[1]] * 3)):
+            with pytest.raises(error):
+                paged_serve.generate(paged, bad, 4)
+            assert len(paged.free) == 12 and not paged.pages and not paged.length
+        with pytest.raises(ValueError):
+            paged_serve.generate(paged, prompts, 4, chunk=0)
+        assert len(paged.free) == 12
+        assert [len(x) for x in paged_serve.generate(paged, prompts, 4)] == [4] * 3
+    finally:
+        paged.release()
+
+
 def test_command_line(capsys):
     from dpuf_b200 import paged_serve
 
