@@ -40,6 +40,7 @@ class PagedModel:
         self.cos, self.sin = serving.rope_table(s.max_seq, s.head_dim, s.rope_theta)
         self.caches = [serving.PagedCache.empty(n_pages, s.n_kv, page_size, s.head_dim, kv_dtype)
                        for _ in range(s.layers)]
+        self.workspace = serving.attention_workspace()
         self.deadzone = float(os.environ.get("DPUF_SWIGLU_DEADZONE", _DEADZONE))
         self.free = list(range(n_pages))
         self.pages: dict[int, list[int]] = {}
@@ -108,7 +109,7 @@ class PagedModel:
             if self.model.has_qk_norm:
                 q, k = self._norm(q, b + "attn_q_norm.weight"), self._norm(k, b + "attn_k_norm.weight")
             q = serving.rope_append(cache, table, q, k, v, self.cos, self.sin, seq_of, pos)
-            o = serving.paged_attention(cache, table, q, q_start, kv_len, max(counts))
+            o = serving.paged_attention(cache, table, q, q_start, kv_len, max(counts), workspace=self.workspace)
             h = h + self._matmul(b + "attn_output.weight", o.flatten(1))
             x = self._norm(h, b + "ffn_norm.weight")
             gate, up = self._matmul(b + "ffn_gate.weight", x), self._matmul(b + "ffn_up.weight", x)
@@ -116,6 +117,7 @@ class PagedModel:
             if self.deadzone > 0:
                 y = torch.where(y.abs() >= self.deadzone, y, 0.0)
             h = h + self._matmul(b + "ffn_down.weight", y)
+        serving.attention_check(workspace=self.workspace)  # (before the new positions count: a step can be repeated)
         for seq, i in batch:
             self.length[seq] += len(i)
         last = self._norm(h[(q_start[1:] - 1).long()], "output_norm.weight")

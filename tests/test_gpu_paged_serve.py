@@ -90,6 +90,26 @@ def test_generate_frees_its_pages_where_a_step_fails():
         paged.release()
 
 
+def test_a_step_says_that_a_wait_gave_up():
+    """The attention's error word set, as a kernel that gave up leaves it: the step raises, and can be repeated."""
+    from dpuf_b200 import paged_serve
+
+    m = mdl.SyntheticModel(mdl.TINY, seed=2)
+    paged = paged_serve.PagedModel(m, 12)
+    try:
+        s = paged.open()
+        want = paged.step([(s, [5, 6, 7])])
+        paged.close(s)
+        s = paged.open()
+        paged.workspace[:1] = 1
+        with pytest.raises(RuntimeError, match="gave up"):
+            paged.step([(s, [5, 6, 7])])
+        assert paged.length[s] == 0
+        assert torch.equal(want, paged.step([(s, [5, 6, 7])]))
+    finally:
+        paged.release()
+
+
 def test_command_line(capsys):
     from dpuf_b200 import paged_serve
 
