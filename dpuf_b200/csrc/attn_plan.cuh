@@ -28,6 +28,7 @@ struct AttnArgs {
   DpufPagedAttentionArgs a;
   int group;    // query heads per KV head
   int max_kv;   // positions that a page table row can hold
+  int most_q;   // new tokens of a sequence that are looked at (so that 32 bits count its rows)
   int page_shift;
 };
 
@@ -38,7 +39,7 @@ struct AttnSeq {
 DPUF_DEV AttnSeq attn_seq(const AttnArgs& p, int s) {
   AttnSeq i;
   i.q0 = min(max(p.a.q_start[s], 0), p.a.n_tokens);
-  i.qn = min(min(max(p.a.q_start[s + 1] - i.q0, 0), p.a.n_tokens - i.q0), p.a.max_q);
+  i.qn = min(min(max(p.a.q_start[s + 1] - i.q0, 0), p.a.n_tokens - i.q0), p.most_q);
   i.kv = min(max(p.a.kv_len[s], 0), p.max_kv);
   return i;
 }

@@ -422,6 +422,7 @@ cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t
   p.group = a.n_q / a.kv.n_kv;
   p.page_shift = 31 - __builtin_clz((unsigned)a.kv.page_size);
   p.max_kv = (int)std::min<int64_t>((int64_t)a.pages_per_seq << p.page_shift, 1 << 30);
+  p.most_q = std::min(1 << 24, (1 << 30) / p.group);
   if (a.kv.dtype == DPUF_TYPE_F32) {
     // up to 4 rows stream (64 tokens at 2,304, 32 / 8 heads of 128: 220 us; by the 16-row tiles 680)
     if (a.max_q * p.group <= kFewRows && a.kv.head_dim <= 128) {

@@ -597,6 +597,25 @@ def test_attention_rows_of_no_sequence(types, q_len, hd):
     assert bool((out == 0).all())
 
 
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("max_q", [1, 5, 100000])
+def test_attention_max_q_that_is_not_the_longest(types, hd, max_q):
+    """max_q chooses the kernel; sequences with more tokens than it says are computed all the same."""
+    g = gen(hd + max_q)
+    q_lens, lens = [1, 40, 7, 150], [30, 61, 7, 400]
+    table, n_pages = table_for(lens, 16, g)
+    cache = serving.PagedCache(*(normal(g, n_pages, 2, 16, hd, dtype=types[1]) for _ in range(2)))
+    start = [0, 1, 41, 48, 198]
+    q = normal(g, 198, 4, hd, dtype=types[0])
+    for window in (0, 33):
+        out = torch.full_like(q, math.nan)
+        serving.paged_attention(cache, table, q, torch.tensor(start, dtype=INT, device="cuda"),
+                                torch.tensor(lens, dtype=INT, device="cuda"), max_q, window=window, out=out)
+        want, bound = attention64(cache, table, q, start, lens, hd ** -0.5, True, window)
+        assert bool(((out.double() - want).abs() <= bound).all())
+
+
 def test_attention_lengths_that_do_not_fit():
     """Lengths and starts are read on the device: ones beyond the table or the tokens are cut off."""
     cache, table, q, start, kv, _ = attention_inputs()
