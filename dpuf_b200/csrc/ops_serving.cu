@@ -29,10 +29,10 @@ bool known_type(int t) { return t == DPUF_TYPE_F32 || t == DPUF_TYPE_F16 || t ==
 int type_bytes(int t) { return t == DPUF_TYPE_F32 ? 4 : 2; }
 bool aligned(const void* p, int n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) == 0; }
 
-// "" or what is wrong with the cache and its table.
+// "" or what is wrong with the cache and its table (which a call without tokens need not have).
 std::string check_cache(const DpufPagedKv& kv, const int32_t* table, int64_t table_stride, int n_seqs,
-                        int pages_per_seq) {
-  if (!kv.k || !kv.v || !table) return "null cache or page table";
+                        int pages_per_seq, int n_tokens) {
+  if (!kv.k || !kv.v || (!table && n_tokens != 0)) return "null cache or page table";
   if (!known_type(kv.dtype)) return "unknown cache type";
   if (kv.n_pages <= 0 || kv.n_kv <= 0) return "a cache needs pages and heads";
   if (kv.page_size < 8 || kv.page_size > 1024 || (kv.page_size & (kv.page_size - 1)))
@@ -43,7 +43,8 @@ std::string check_cache(const DpufPagedKv& kv, const int32_t* table, int64_t tab
       kv.row_stride * b % 16)
     return "the cache's bases and strides must be multiples of 16 bytes";
   if (kv.page_stride < 0 || kv.head_stride < 0 || kv.row_stride < kv.head_dim) return "bad cache strides";
-  if (n_seqs <= 0 || pages_per_seq <= 0 || table_stride < pages_per_seq) return "bad page table shape";
+  const int least = n_tokens != 0 ? 1 : 0;
+  if (n_seqs < least || pages_per_seq < least || table_stride < pages_per_seq) return "bad page table shape";
   return "";
 }
 
@@ -59,7 +60,7 @@ DPUF_EXPORT int32_t dpuf_cuda_rope_append(const DpufRopeAppendArgs* args, void* 
   set_error("");
   if (!args) return refuse(me, "null arguments");
   const DpufRopeAppendArgs& a = *args;
-  const std::string bad = check_cache(a.kv, a.page_table, a.table_stride, a.n_seqs, a.pages_per_seq);
+  const std::string bad = check_cache(a.kv, a.page_table, a.table_stride, a.n_seqs, a.pages_per_seq, a.n_tokens);
   if (!bad.empty()) return refuse(me, bad);
   if (a.n_tokens < 0) return refuse(me, "negative n_tokens");
   if (a.n_tokens == 0) return 0;
@@ -85,7 +86,7 @@ DPUF_EXPORT int32_t dpuf_cuda_paged_attention(const DpufPagedAttentionArgs* args
   set_error("");
   if (!args) return refuse(me, "null arguments");
   DpufPagedAttentionArgs a = *args;
-  const std::string bad = check_cache(a.kv, a.page_table, a.table_stride, a.n_seqs, a.pages_per_seq);
+  const std::string bad = check_cache(a.kv, a.page_table, a.table_stride, a.n_seqs, a.pages_per_seq, a.n_tokens);
   if (!bad.empty()) return refuse(me, bad);
   if (a.n_tokens < 0) return refuse(me, "negative n_tokens");
   if (a.n_tokens == 0) return 0;

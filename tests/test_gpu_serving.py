@@ -632,6 +632,20 @@ def test_attention_lengths_that_do_not_fit():
     assert bool((serving.paged_attention(cache, table, q, start, kv2, 1)[0] == 0).all())
 
 
+@pytest.mark.parametrize("seqs,width", [(0, 4), (0, 0), (3, 0), (3, 4)])
+def test_a_batch_without_tokens(seqs, width):
+    cache = serving.PagedCache.empty(4, 2, 16, 64)
+    table = torch.zeros(seqs, width, dtype=INT, device="cuda")
+    q, k = torch.zeros(0, 4, 64, dtype=F16, device="cuda"), torch.zeros(0, 2, 64, dtype=F16, device="cuda")
+    cos, sin = serving.rope_table(8, 64)
+    none = torch.zeros(0, dtype=INT, device="cuda")
+    assert serving.rope_append(cache, table, q, k, k, cos, sin, none, none).shape == (0, 4, 64)
+    start, kv = torch.zeros(seqs + 1, dtype=INT, device="cuda"), torch.zeros(seqs, dtype=INT, device="cuda")
+    assert serving.paged_attention(cache, table, q, start, kv, 1).shape == (0, 4, 64)
+    ids, probs = serving.sample(torch.zeros(0, 100, device="cuda"), torch.zeros(0, device="cuda"))
+    assert ids.shape == probs.shape == (0,)
+
+
 def test_attention_refusals():
     cache, table, q, start, kv, n = attention_inputs()
     ok = (cache, table, q, start, kv, n)

@@ -93,6 +93,17 @@ def test_empty_calls_do_nothing(lib):
         assert fn(None, None) == -1
 
 
+def test_a_batch_of_no_sequences_does_nothing(lib):
+    """No tokens of no sequences: a table of no rows or no entries, whose tensor has no address."""
+    for over in (dict(seqs=0), dict(width=0, tstride=0), dict(seqs=0, width=0, tstride=0)):
+        assert lib.dpuf_cuda_rope_append(rope_args(n=0, table=0, **over), None) == 0
+        assert lib.dpuf_cuda_paged_attention(attn_args(n=0, table=0, **over), None) == 0
+        assert lib.dpuf_cuda_rope_append(rope_args(kv(n_kv=0), n=0, table=0, **over), None) == -1
+        assert lib.dpuf_cuda_paged_attention(attn_args(kv(n_kv=0), n=0, table=0, **over), None) == -1
+    assert lib.dpuf_cuda_rope_append(rope_args(n=0, table=0, seqs=-1), None) == -1
+    assert lib.dpuf_cuda_paged_attention(attn_args(n=0, table=0, width=-1), None) == -1
+
+
 def test_cache_refuses_host_tensors():
     x = torch.zeros(2, 2, 16, 64, dtype=torch.float16)
     with pytest.raises(ValueError):
