@@ -424,7 +424,10 @@ cudaError_t launch_paged_attention(const DpufPagedAttentionArgs& a, cudaStream_t
   p.max_kv = (int)std::min<int64_t>((int64_t)a.pages_per_seq << p.page_shift, 1 << 30);
   p.most_q = std::min(1 << 24, (1 << 30) / p.group);
   if (a.kv.dtype == DPUF_TYPE_F32) {
-    // up to 4 rows stream (64 tokens at 2,304, 32 / 8 heads of 128: 220 us; by the 16-row tiles 680)
+    // Up to 4 rows, one tile of the streaming kernel (64 tokens at 2,304, 32 / 8 heads of 128: 220 us; by
+    // the 16-row tiles 680).  More rows would read the keys once per 4 and still take less up to about 14
+    // (from a flushed L2: 7 rows, 28 / 4 heads, 231 us against 395; 8, 16 / 2 heads, 128 and 209; 16,
+    // 16 / 1 heads, 137 and 129): the limit is not where the two meet.
     if (a.max_q * p.group <= kFewRows && a.kv.head_dim <= 128) {
       if (a.kv.head_dim <= 64)
         paged_attention_f32_few_kernel<64><<<kAttnSms * few_ctas(64), kFewWarps * 32, 0, s>>>(p);

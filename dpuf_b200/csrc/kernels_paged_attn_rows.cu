@@ -12,6 +12,11 @@
 // the cache's type (2 of fp16 carry 22 bits, 3 of bf16 24), and so are the weights; each product
 // is kTerms MMAs.  The weights carry a factor 2^12, which the sum carries too, so that in fp16 the
 // small ones of a long context keep their bits (a weight of 2^-26 of the largest is still normal).
+//
+// 16-bit queries take their weights in one term, rounded to the cache's type (the sum keeps them
+// unrounded): the output is rounded to that type once more anyway, and the largest weight, a power
+// of two, is exact.  Relative errors against 64 bits, and of the output's rounding alone: 64 tokens
+// at 2,304 in fp16 2.15e-4 and 2.07e-4; one at 131,071 in bf16 1.68e-3 and 1.66e-3.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 

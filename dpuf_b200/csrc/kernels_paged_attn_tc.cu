@@ -10,7 +10,11 @@
 //                     and scales O in TMEM only when its row's maximum has grown by more than 2^8
 //                     since the last time (weights are then at most 2^8, which both types hold with
 //                     their full precision; the division by the sum at the end makes up for it),
-//                     which after the first blocks is rare.
+//                     which after the first blocks is rare.  P has 16 bits because the MMA takes A
+//                     and B of one type; a second term would be half as much again of tensor work.
+//                     Relative errors against 64 bits, and of the output's rounding alone: four
+//                     prompts of 2,048 in fp16 2.7e-4 and 2.1e-4, 512 tokens over 33,280 in bf16
+//                     2.1e-3 and 1.7e-3.
 //   warp 8            TMA: 64-column boxes of a page's rows (128-byte swizzle) into a ring of key
 //                     and value blocks; a page that is not held, or that no row sees, is a box
 //                     outside the tensor and arrives as zeros.
@@ -49,6 +53,8 @@ constexpr int kKeys = 64;             // of a block
 constexpr int kItemRows = 2 * kTile;
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kQueryWarp = 11;  // kMmaWarp + i: tile i
 constexpr int kThreads = 384;
+// (The figures of these three are of one input in short bursts; with inputs in rotation, where power
+// limits the clock, four prompts of 2,048 take 183 to 189 us.)
 // What an item costs beside its blocks, in blocks (four prompts of 2,048: 178 us at 0, 167 at 2, 168 at 3, 174 at 5).
 constexpr int kLead = 2;
 // Cuts that move to an item's end (a part of 256 rows is 128 KB out and in again).  49 x 216 tokens

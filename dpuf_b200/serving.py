@@ -331,7 +331,8 @@ def attention_check(device: int | None = None, workspace: torch.Tensor | None = 
     call on the workspace (without one, the stream's) gave up since the last check: the outputs of that
     call and of those after it are undefined.  The workspace is then ready for use again."""
     dev = torch.cuda.current_device() if device is None else device
-    _call(_lib().dpuf_cuda_paged_attention_status, dev, (_workspace(dev) if workspace is None else _given(workspace, dev))[1])
+    ws = _workspace(dev) if workspace is None else _given(workspace, dev)
+    _call(_lib().dpuf_cuda_paged_attention_status, dev, ws[1])
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None,
