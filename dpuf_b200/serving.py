@@ -284,7 +284,7 @@ def paged_attention(cache: PagedCache, page_table: torch.Tensor, q: torch.Tensor
     Sequence s (row s of page_table) has the new tokens q_start[s] .. q_start[s + 1] (int32
     `[sequences + 1]`, ascending), which are the last of its kv_len[s] (int32) positions and have been
     appended; tokens before q_start[0] and from the last entry on are padding and get zeros.  max_q, the
-    most new tokens of a sequence, chooses the kernel (results do not hang on it).  A token at position
+    most new tokens of a sequence, chooses the kernel (results differ by rounding alone).  A token at position
     p sees the positions up to p (all kv_len[s] where not causal), with `window` > 0 the last `window`
     of them; one that sees nothing gets zeros.
     n_q is a multiple of the cache's heads.  q is float32 or of the cache's type and may be a slice

@@ -220,7 +220,7 @@ DPUF_EXPORT int32_t dpuf_cuda_rope_append(const DpufRopeAppendArgs* args, void* 
  *   out = sum_j softmax_j(scale * q . k_j) v_j,
  * zeros for a token that sees nothing.  Query head h reads KV head h / (n_q / n_kv).  max_q (the
  * largest q_start[s+1] - q_start[s], which the host need not wait for: another value costs time
- * and not results) chooses the kernel; a sequence has at most 2^24 new tokens, and 2^30 rows
+ * and no more than rounding) chooses the kernel; a sequence has at most 2^24 new tokens, and 2^30 rows
  * (tokens x n_q / n_kv).  dtype is that of q and is float32 or the cache's, out_dtype that of out
  * [n_tokens][n_q][head_dim] (contiguous) and is dtype or float32.  Positions that no token of a
  * sequence sees are never used, whatever stands there; a value that is not finite at a position
